@@ -451,6 +451,60 @@ int mn_conv_bwd_weight_bias(const mn_conv2d* g, const void* dy, const void* x, v
                             void* ws, size_t ws_bytes, int variant, int dtype,
                             mn_stream_t stream);
 
+/* ------------------------------------------------------- transformer block --
+ * The operators between the linear layers of a transformer block.  The
+ * reference has none of them ; they follow the contract of its
+ * operator classes (monet/lm_ops/base.py:2-53), in which a backward
+ * names the few tensors it needs kept.
+ *
+ * `dtype` is the type of activations and their gradients: MN_F32, MN_BF16 or
+ * MN_F16, row-major (the channels-last rule of MN_BF16 above concerns
+ * convolutions only).  Rows may start at any address that is a multiple of the
+ * element size.  All sums are fp32; a result is rounded once. */
+#define MN_F16 2
+
+/* y = (x - mean) * rstd * w + b per row of D elements; w, b may be NULL (1, 0).
+ * wdtype: type of w and b, `dtype` or MN_F32.  mean / rstd [rows] may be NULL.
+ * y may alias x. */
+int mn_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
+                      int64_t rows, int64_t D, double eps, int dtype, int wdtype, mn_stream_t stream);
+/* Workspace of mn_layer_norm_bwd (4-byte aligned), needed when dw or db is asked for. */
+size_t mn_layer_norm_ws_bytes(int64_t rows, int64_t D);
+/* dx, dw, db; each may be NULL, dx may alias grad.  dw and db have wdtype; their sums over the
+ * rows run in a fixed order (no atomics).  rows == 0 gives dw = db = 0. */
+int mn_layer_norm_bwd(const void* grad, const void* x, const float* mean, const float* rstd,
+                      const void* w, void* dx, void* dw, void* db, int64_t rows, int64_t D, int dtype,
+                      int wdtype, void* ws, size_t ws_bytes, mn_stream_t stream);
+
+/* y[e] = u(e) >= round(p * 2^32) ? x[e] / (1 - p) : 0 with u(e) a 32-bit number that depends on
+ * state = {seed, offset} (device memory) and e alone: the same call on the gradient is the
+ * backward pass, and a repeated forward drops the same elements.  Element e takes the 16-bit
+ * piece e % 8 (low half of a word before the high one) of Philox4x32-10 at counter
+ * (g, g >> 32, offset, offset >> 32), g = e / 8, key seed, as the high half of u(e), and the same
+ * piece at counter (g, g >> 32 | 2^31, ...) as its low half.  0 <= p <= 1; y may alias x. */
+int mn_dropout(const void* x, void* y, int64_t n, double p, const uint64_t* state, int dtype,
+               mn_stream_t stream);
+
+/* Rotary positions: x [B, T, H, D] with strides in elements (the last one is 1), y dense.  Axis a
+ * (of `axes`, at most 3) turns sections[a] pairs; pair i of axis a, i-th of the axis and k-th of
+ * all n = sum(sections), by the angle pos[a, b, t] * base^(-i / sections[a]), or base^(-k / n) if
+ * `joint`.  Pairs are elements (k, k + n), or (2k, 2k + 1) if `interleaved`; elements from 2n on
+ * are copied.  n <= 128, H * D < 2^24.  inverse != 0 turns back: the backward pass. */
+#define MN_POS_I64 0
+#define MN_POS_I32 1
+#define MN_POS_F32 2
+typedef struct mn_rotary_desc {
+  int64_t B, T;
+  int32_t H, D;
+  int32_t axes, sections[3];
+  int32_t joint, interleaved, pos_type, reserved;
+  double base;
+  int64_t x_stride[3];   /* b, t, h */
+  int64_t pos_stride[3]; /* axis, b (0: the batch shares positions), t */
+} mn_rotary_desc;
+int mn_rotary(const mn_rotary_desc* d, const void* x, const void* positions, void* y, int inverse,
+              int dtype, mn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

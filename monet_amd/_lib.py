@@ -5,8 +5,8 @@ caller gets an exception, never a fallback.
 """
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64,
-                    c_size_t, c_uint32, c_void_p)
+from ctypes import (POINTER, Structure, byref, c_char_p, c_double, c_float, c_int,
+                    c_int32, c_int64, c_size_t, c_uint32, c_void_p)
 from pathlib import Path
 
 import torch
@@ -37,12 +37,22 @@ class Conv2d(Structure):
 CONV_FWD, CONV_BWD_DATA, CONV_BWD_WEIGHT = 0, 1, 2
 F32 = 0
 BF16 = 1   # bf16 tensors in channels-last order (see include/monet_hip.h)
+F16 = 2    # transformer-block operators only
+DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 
 class Pool2d(Structure):
     """Mirror of `struct mn_pool2d`."""
     _fields_ = [(k, c_int32) for k in
                 ("N", "C", "H", "W", "kH", "kW", "sH", "sW", "pH", "pW", "dH", "dW", "PH", "PW")]
+
+
+class RotaryDesc(Structure):
+    """Mirror of `struct mn_rotary_desc`."""
+    _fields_ = [("B", c_int64), ("T", c_int64), ("H", c_int32), ("D", c_int32), ("axes", c_int32),
+                ("sections", c_int32 * 3), ("joint", c_int32), ("interleaved", c_int32),
+                ("pos_type", c_int32), ("reserved", c_int32), ("base", c_double),
+                ("x_stride", c_int64 * 3), ("pos_stride", c_int64 * 3)]
 
 
 _P = c_void_p
@@ -109,6 +119,12 @@ _SIGNATURES = {
     "mn_conv_bwd_weight": (c_int, [POINTER(Conv2d), _P, _P, _P, _P, c_size_t, c_int, c_int, _P]),
     "mn_conv_bwd_weight_bias": (c_int, [POINTER(Conv2d), _P, _P, _P, _P, _P, c_size_t, c_int, c_int,
                                         _P]),
+    "mn_layer_norm_fwd": (c_int, [_P, _P, _P, _P, _P, _P, c_int64, c_int64, c_double, c_int, c_int, _P]),
+    "mn_layer_norm_ws_bytes": (c_size_t, [c_int64, c_int64]),
+    "mn_layer_norm_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int, c_int, _P,
+                                  c_size_t, _P]),
+    "mn_dropout": (c_int, [_P, _P, c_int64, c_double, _P, c_int, _P]),
+    "mn_rotary": (c_int, [POINTER(RotaryDesc), _P, _P, _P, c_int, c_int, _P]),
 }
 # entry points whose int return value is NOT a status code
 _UNCHECKED = {"mn_abi_version", "mn_conv_n_variants", "mn_conv_n_variants_for"}
@@ -177,3 +193,25 @@ def require_gpu_tensor(t, name, dtype=None):
     if dtype is not None and t.dtype != dtype:
         raise RuntimeError(f"{name} must have dtype {dtype}, got {t.dtype}")
     return t
+
+
+def require_same_device(x, t, name):
+    if t.device != x.device:
+        raise RuntimeError(f"{name} is on {t.device}, the input on {x.device}")
+
+
+def dtype_code(t, name):
+    """MN_F32 / MN_BF16 / MN_F16 of a GPU tensor."""
+    require_gpu_tensor(t, name)
+    code = DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{name} must have dtype float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def call_on(device, name, *args):
+    """`call` with `device` current and its current stream as the last argument."""
+    if device.index == torch.cuda.current_device():
+        return call(name, *args, stream_ptr(device))
+    with torch.cuda.device(device):
+        return call(name, *args, stream_ptr(device))

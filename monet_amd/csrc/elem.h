@@ -1,0 +1,58 @@
+// Element types and unaligned vector access shared by the kernels that take fp32, bf16 and fp16
+// tensors (layer norm, dropout, rotary positions, attention).
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// 16 bytes of T.  The alignment of one element is enough: rows of odd length and views that
+// start anywhere take the same 16-byte global accesses (the hardware splits the ones that cross
+// a line), so no kernel has an aligned and an unaligned variant.
+template <typename T>
+struct Vec16 {
+  static constexpr int N = 16 / (int)sizeof(T);
+  typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef T utype __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+// `cnt` (0..N) elements from p as fp32, zeros behind them.
+template <typename T>
+__device__ __forceinline__ void load_vec(const T* p, int cnt, float* out) {
+  constexpr int N = Vec16<T>::N;
+  if (cnt == N) {
+    const typename Vec16<T>::utype v = *reinterpret_cast<const typename Vec16<T>::utype*>(p);
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = e < cnt ? (float)p[e] : 0.f;
+  }
+}
+
+// The first `cnt` (0..N) of N fp32 values to p, rounded once to nearest even.
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, int cnt, const float* in) {
+  constexpr int N = Vec16<T>::N;
+  if (cnt == N) {
+    typename Vec16<T>::utype v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = (T)in[e];
+    *reinterpret_cast<typename Vec16<T>::utype*>(p) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < cnt) p[e] = (T)in[e];
+  }
+}
+
+// Calls f with a value of the element type that `dtype` names; MN_EUNSUPPORTED for others.
+template <typename F>
+static inline int mn_for_dtype(int dtype, F f) {
+  switch (dtype) {
+    case MN_F32: return f(float());
+    case MN_BF16: return f(bf16_t());
+    case MN_F16: return f(f16_t());
+    default: return MN_EUNSUPPORTED;
+  }
+}

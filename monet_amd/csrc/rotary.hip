@@ -1,0 +1,190 @@
+// Rotary positions over several axes (row and column of an image's patches, frame of a video).
+//
+// The first 2*n elements of a head are n pairs, (i, i+n) or, interleaved, (2i, 2i+1); pair i is
+// turned by the angle position[axis(i)] * frequency(i), the rest is copied.  Backward turns the
+// other way, so it is the same kernel with the sign of the sine changed.
+//
+// Bound by memory: one read, one write.  What could cost more are the angles: they are needed
+// once per (token, pair) but used by every head and, where positions do not depend on the batch,
+// by every batch entry, so a workgroup makes a table of cosines and sines for TOK tokens in LDS
+// and walks over heads and entries of the batch with it.
+// Angles are held in TURNS in 64 bits: position * (frequency / 2 pi) leaves its whole turns and
+// quarter turns exactly (what is left is at most an eighth of a turn, 2^-28 turns after rounding
+// to fp32), so a position of a million is as accurate as position 1; sine and cosine of that rest
+// are fp32.
+#include <math.h>
+
+#include "elem.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPairs = 128;
+constexpr int64_t kMaxToken = 1 << 24;   // elements of a token
+constexpr int kTableFloats = 8192;   // 32 KB of LDS: TOK * pairs * 2
+
+struct Rotary {
+  double turns[kMaxPairs];    // frequency / (2 pi)
+  uint8_t axis[kMaxPairs];
+  int64_t B, T;
+  int64_t sxb, sxt, sxh;      // strides of x in elements
+  int64_t spa, spb, spt;      // strides of the positions
+  int32_t H, D, n, tok, bchunk;
+  float sign;
+};
+
+template <typename P>
+__device__ __forceinline__ float2_t cos_sin(P pos, double turns) {
+  double t = (double)pos * turns;
+  t -= rint(t);                                  // [-1/2, 1/2]
+  const double quarter = rint(4.0 * t);          // -2 .. 2
+  const float rest = (float)(t - 0.25 * quarter) * 2.f;   // half turns, |rest| <= 1/4
+  float s, c;
+  sincospif(rest, &s, &c);
+  switch ((int)quarter & 3) {
+    case 0: return float2_t{c, s};
+    case 1: return float2_t{-s, c};
+    case 2: return float2_t{-c, -s};
+    default: return float2_t{s, -c};
+  }
+}
+
+template <typename T, typename P, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const T* __restrict__ x, T* __restrict__ y,
+                                                          const P* __restrict__ pos, const Rotary a) {
+  constexpr int N = Vec16<T>::N;
+  extern __shared__ float2_t table[];   // [tok][n]
+  const int64_t t0 = (int64_t)blockIdx.x * a.tok, b0 = (int64_t)blockIdx.y * a.bchunk;
+  const int toks = a.T - t0 < a.tok ? (int)(a.T - t0) : a.tok;
+  const int batches = a.B - b0 < a.bchunk ? (int)(a.B - b0) : a.bchunk;
+  for (int i = threadIdx.x; i < toks * a.n; i += kThreads) {
+    const int t = i / a.n, k = i - t * a.n;
+    float2_t cs = cos_sin<P>(pos[a.axis[k] * a.spa + b0 * a.spb + (t0 + t) * a.spt], a.turns[k]);
+    cs[1] *= a.sign;
+    table[i] = cs;
+  }
+  __syncthreads();
+  // units of a head: chunks of pairs (N pairs, or N / 2 interleaved), then chunks that are copied
+  const int per = INTERLEAVED ? N / 2 : N;
+  const int pair_units = (a.n + per - 1) / per, rest = a.D - 2 * a.n;
+  const int units = pair_units + (rest + N - 1) / N;
+  const uint32_t per_token = (uint32_t)a.H * units;
+  const uint32_t total = (uint32_t)batches * toks * per_token;
+  for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
+    const uint32_t bt = i / per_token, hu = i - bt * per_token;
+    const int h = hu / units, u = hu - h * units;
+    const uint32_t bi = bt / toks;
+    const int t = bt - bi * toks;
+    const int64_t b = b0 + bi;
+    const T* xr = x + b * a.sxb + (t0 + t) * a.sxt + h * a.sxh;
+    T* yr = y + ((b * a.T + t0 + t) * a.H + h) * a.D;
+    if (u >= pair_units) {
+      const int col = 2 * a.n + (u - pair_units) * N;
+      const int cnt = a.D - col < N ? a.D - col : N;
+      float v[N];
+      load_vec<T>(xr + col, cnt, v);
+      store_vec<T>(yr + col, cnt, v);
+      continue;
+    }
+    const int p0 = u * per, pairs = a.n - p0 < per ? a.n - p0 : per;
+    const float2_t* cs = table + t * a.n + p0;
+    float v[N], w[N];
+    if (INTERLEAVED) {
+      load_vec<T>(xr + 2 * p0, 2 * pairs, v);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        if (e >= pairs) break;
+        const float2_t c = cs[e];
+        w[2 * e] = v[2 * e] * c[0] - v[2 * e + 1] * c[1];
+        w[2 * e + 1] = v[2 * e] * c[1] + v[2 * e + 1] * c[0];
+      }
+      store_vec<T>(yr + 2 * p0, 2 * pairs, w);
+    } else {
+      load_vec<T>(xr + p0, pairs, v);
+      load_vec<T>(xr + a.n + p0, pairs, w);
+      float lo[N], hi[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (e >= pairs) break;
+        const float2_t c = cs[e];
+        lo[e] = v[e] * c[0] - w[e] * c[1];
+        hi[e] = v[e] * c[1] + w[e] * c[0];
+      }
+      store_vec<T>(yr + p0, pairs, lo);
+      store_vec<T>(yr + a.n + p0, pairs, hi);
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int mn_rotary(const mn_rotary_desc* d, const void* x, const void* positions, void* y, int inverse,
+              int dtype, mn_stream_t stream) {
+  if (!d) return MN_EINVAL;
+  if (d->B < 0 || d->T < 0 || d->H < 0 || d->D <= 0 || d->axes < 1 || d->axes > 3 || !(d->base > 0.0))
+    return MN_EINVAL;
+  int64_t n = 0;
+  for (int k = 0; k < d->axes; ++k) {
+    if (d->sections[k] < 0) return MN_EINVAL;
+    n += d->sections[k];
+  }
+  if (2 * n > d->D) return MN_EINVAL;
+  if (n > kMaxPairs || (int64_t)d->H * d->D >= kMaxToken || d->B >= (1ll << 31) || d->T >= (1ll << 31))
+    return MN_EUNSUPPORTED;
+  if (d->pos_type < MN_POS_I64 || d->pos_type > MN_POS_F32) return MN_EUNSUPPORTED;
+  Rotary a = {};
+  int k = 0;
+  for (int axis = 0; axis < d->axes; ++axis)
+    for (int i = 0; i < d->sections[axis]; ++i, ++k) {
+      const double power = d->joint ? (double)k / (double)n : (double)i / (double)d->sections[axis];
+      a.turns[k] = pow(d->base, -power) * 0.15915494309189533577;   // 1 / (2 pi)
+      a.axis[k] = (uint8_t)axis;
+    }
+  a.B = d->B; a.T = d->T; a.H = d->H; a.D = d->D; a.n = (int)n;
+  a.sxb = d->x_stride[0]; a.sxt = d->x_stride[1]; a.sxh = d->x_stride[2];
+  a.spa = d->pos_stride[0]; a.spb = d->pos_stride[1]; a.spt = d->pos_stride[2];
+  a.sign = inverse ? -1.f : 1.f;
+  // tokens of a workgroup: about 16 KB of x in all, as far as the table has room; entries of the
+  // batch share the table unless their positions differ, as long as 2048 workgroups remain
+  const int64_t token_elems = (int64_t)a.H * a.D;
+  int64_t tok = token_elems ? 8192 / token_elems : 1;
+  const int64_t room = n ? kTableFloats / (2 * n) : 64;
+  tok = tok < 1 ? 1 : (tok > room ? room : (tok > 64 ? 64 : tok));
+  if (tok > a.T) tok = a.T > 0 ? a.T : 1;
+  a.tok = (int)tok;
+  const int64_t tblocks = (a.T + tok - 1) / tok;
+  int64_t bchunk = 1;
+  if (a.spb == 0) {
+    bchunk = a.B * tblocks / 2048;
+    bchunk = bchunk < 1 ? 1 : bchunk;
+  }
+  // (the grid's second dimension ends at 65535, a workgroup's elements are counted in 32 bits)
+  while ((a.B + bchunk - 1) / bchunk > 65535 && a.spb == 0) bchunk *= 2;
+  const int64_t most = token_elems ? (1ll << 31) / (tok * token_elems) - 1 : bchunk;
+  if (bchunk > most) bchunk = most;
+  if ((a.B + bchunk - 1) / bchunk > 65535) return MN_EUNSUPPORTED;
+  a.bchunk = (int)(bchunk < a.B ? bchunk : a.B);
+  return mn_for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (a.B == 0 || a.T == 0 || a.H == 0) return (int)MN_OK;
+    if (!x || !positions || !y) return (int)MN_EINVAL;
+    const dim3 grid((unsigned)tblocks, (unsigned)((a.B + a.bchunk - 1) / a.bchunk));
+    const size_t lds = (size_t)a.tok * a.n * sizeof(float2_t);
+    hipStream_t s = mn_stream(stream);
+    const auto launch = [&](auto p) {
+      using P = decltype(p);
+      if (d->interleaved)
+        rotary_kernel<T, P, true><<<grid, kThreads, lds, s>>>((const T*)x, (T*)y, (const P*)positions, a);
+      else
+        rotary_kernel<T, P, false><<<grid, kThreads, lds, s>>>((const T*)x, (T*)y, (const P*)positions, a);
+      return mn_launch_status();
+    };
+    if (d->pos_type == MN_POS_I64) return launch(int64_t());
+    if (d->pos_type == MN_POS_I32) return launch(int32_t());
+    return launch(float());
+  });
+}
+
+}  // extern "C"
