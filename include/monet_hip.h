@@ -43,7 +43,8 @@ const char* mn_status_string(int status);
 /* Optional.  Does now, for the CURRENT device, what a few entry points would
  * otherwise do on their first call there and what is not a stream operation:
  * looks up the address of the fixed workspace of mn_bn_bwd_from_y_static_f32
- * and raises the LDS limit of the one-kernel Winograd convolution.  A caller
+ * and raises the LDS limits of the one-kernel Winograd convolution and of
+ * attention.  A caller
  * that captures HIP graphs calls it once per device before the first capture
  * (or makes one call of those entry points outside capture); everyone else may
  * ignore it.  Idempotent, thread-safe; MN_ELAUNCH if a lookup fails.  No
@@ -504,6 +505,33 @@ typedef struct mn_rotary_desc {
 } mn_rotary_desc;
 int mn_rotary(const mn_rotary_desc* d, const void* x, const void* positions, void* y, int inverse,
               int dtype, mn_stream_t stream);
+
+/* Attention of T queries over the T keys of the same sequence; query head h reads key head
+ * h / (Hq / Hkv).  Query i sees key j if
+ *     j <= i + right  and  (j >= i - left  or  j < sinks)  and  i, j < lengths[b];
+ * left / right = -1: no limit; right = 0: nothing later.  `lengths` (int32 [B], device) may be
+ * NULL (T everywhere); tokens from lengths[b] on are never read as keys, and their own outputs
+ * and gradients are zeros (lse -inf), whatever their memory holds.
+ * q [B, T, Hq, D], k and v [B, T, Hkv, D] with strides in elements (the last one is 1); every
+ * other tensor is dense: out, grad, dq [B, T, Hq, D], dk, dv [B, T, Hkv, D], lse fp32 [B, Hq, T],
+ * the natural logarithm of the sum of exp(scale * q k).  D <= 128, scale > 0.  16-bit types
+ * multiply 16-bit operands (P and dS are rounded to the type) and add in fp32. */
+typedef struct mn_attention {
+  int64_t B, T;
+  int32_t Hq, Hkv, D, reserved;
+  int64_t left, right, sinks;
+  float scale, reserved2;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* b, t, h */
+} mn_attention;
+int mn_attention_fwd(const mn_attention* d, const void* q, const void* k, const void* v,
+                     const int32_t* lengths, void* out, float* lse, int dtype, mn_stream_t stream);
+/* Workspace of mn_attention_bwd (4-byte aligned). */
+size_t mn_attention_bwd_ws_bytes(const mn_attention* d);
+/* dq, dk, dv from the forward's inputs, out and lse.  No atomics: the same bits every run. */
+int mn_attention_bwd(const mn_attention* d, const void* grad, const void* q, const void* k,
+                     const void* v, const void* out, const float* lse, const int32_t* lengths,
+                     void* dq, void* dk, void* dv, int dtype, void* ws, size_t ws_bytes,
+                     mn_stream_t stream);
 
 #ifdef __cplusplus
 }

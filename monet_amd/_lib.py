@@ -55,6 +55,14 @@ class RotaryDesc(Structure):
                 ("x_stride", c_int64 * 3), ("pos_stride", c_int64 * 3)]
 
 
+class AttentionDesc(Structure):
+    """Mirror of `struct mn_attention`."""
+    _fields_ = [("B", c_int64), ("T", c_int64), ("Hq", c_int32), ("Hkv", c_int32), ("D", c_int32),
+                ("reserved", c_int32), ("left", c_int64), ("right", c_int64), ("sinks", c_int64),
+                ("scale", c_float), ("reserved2", c_float), ("q_stride", c_int64 * 3),
+                ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3)]
+
+
 _P = c_void_p
 _SIGNATURES = {
     # name: (restype, argtypes); restype c_int means "status code, checked"
@@ -124,6 +132,9 @@ _SIGNATURES = {
     "mn_layer_norm_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int, c_int, _P,
                                   c_size_t, _P]),
     "mn_dropout": (c_int, [_P, _P, c_int64, c_double, _P, c_int, _P]),
+    "mn_attention_fwd": (c_int, [POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, c_int, _P]),
+    "mn_attention_bwd_ws_bytes": (c_size_t, [POINTER(AttentionDesc)]),
+    "mn_attention_bwd": (c_int, [POINTER(AttentionDesc)] + [_P] * 10 + [c_int, _P, c_size_t, _P]),
     "mn_rotary": (c_int, [POINTER(RotaryDesc), _P, _P, _P, c_int, c_int, _P]),
 }
 # entry points whose int return value is NOT a status code

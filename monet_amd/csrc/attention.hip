@@ -1,0 +1,741 @@
+// Attention over a sliding window plus a few first tokens ("sinks"), forward and backward, for
+// training: queries and keys of one sequence of T tokens, heads of queries sharing heads of keys.
+//
+//   visible(i, j):  j <= i + right  and  (j >= i - left  or  j < sinks)  and  i, j < length
+//   P = softmax_j(scale q_i k_j),  o = P v,  lse = log sum_j exp(scale q_i k_j)
+//   dv = P^T do,  dP = do v^T,  dS = P (dP - rowsum(do o)),  dq = scale dS k,  dk = scale dS^T q
+//
+// Scores are never stored: forward keeps a running maximum and sum per row, backward computes P
+// again from lse.  All products run on the matrix cores with fp32 accumulators: 16-bit types on
+// 32x32x16 instructions, fp32 on 32x32x2.
+//
+// Orientation.  A 32x32 accumulator holds one COLUMN per lane (lane l: column l % 32, of its 32
+// rows the 16 with bit 2 equal to l / 32).  Scores are computed transposed where a row of the
+// softmax runs over keys (S^T = K Q^T: a lane owns one query, so maximum and sum are a fold over
+// registers and one exchange with lane l ^ 32), and the accumulator's registers are, in order,
+// the B operand of the next product over the same 32 keys (or queries): which of the 32 a slot of
+// the contraction means is free as long as A uses the same assignment, and the A operand is read
+// from LDS for exactly those.  P and dS therefore never leave the registers of their lane.
+//
+// LDS tiles hold rows of D elements as they lie in memory; 16-byte chunk c of row r is stored at
+// chunk c ^ swz(r), which spreads both kinds of reads over all banks: rows (a lane reads 16 bytes
+// of its row) and transposed (16-bit: ds_read_b64_tr_b16 gives a lane four rows' values of its
+// column; fp32: plain 4-byte reads).
+#include "elem.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / MN_WAVE;
+constexpr int kMaxD = 128;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct Args {
+  const void *q, *k, *v, *out, *grad;   // out, grad: dense [B, T, Hq, D]
+  void *o, *dq, *dk, *dv;               // dense results
+  float *lse;                           // [B, Hq, T]
+  float *delta;                         // [B, Hq, T] rowsum(do * o), written by the dq kernel
+  float *parts;                         // partial dk, dv of key tiles that are split over queries
+  const int32_t* lengths;
+  int64_t sq[3], sk[3], sv[3];          // strides of b, t, h in elements
+  int32_t T, Hq, Hkv, D, left, right, sinks;
+  int32_t tiles, group;
+  int32_t sink_tiles, chunk, nchunks;   // dk / dv: see there
+  float scale, scale_log2;
+};
+
+// ------------------------------------------------------------------------- matrix-core types
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16_t> {
+  typedef bf16_t frag __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<f16_t> {
+  typedef f16_t frag __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {   // four contraction slots a lane: four instructions of two
+  typedef float frag __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// One tile of rows in LDS: DP elements a row (D rounded up to 32, zeros behind D).
+template <typename T, int DP, int ROWS>
+struct Tile {
+  typedef typename Mma<T>::frag frag;
+  static constexpr int N = 16 / (int)sizeof(T);      // elements of a chunk
+  static constexpr int CH = DP / N;                  // chunks of a row that hold data
+  static constexpr int NC = CH <= 4 ? 4 : CH <= 8 ? 8 : CH <= 16 ? 16 : 32;   // chunks of a row
+  static constexpr int STEPS = CH / 2;               // steps of a contraction over D
+  static constexpr int BYTES = ROWS * NC * 16;
+  static constexpr int PER = ROWS * CH / kThreads;   // chunks a thread stages
+  static_assert(ROWS * CH % kThreads == 0, "whole chunks per thread");
+
+  static __device__ __forceinline__ int swz(int row) {
+    if (NC >= 16) return (row & 3) << 2 | (row >> 2 & 3);
+    if (NC == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    return row >> 2 & 3;
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return (row * NC + (chunk ^ swz(row))) * 16;
+  }
+
+  // global -> registers: rows r0 .. r0 + ROWS of a head, rows from `end` on as zeros
+  static __device__ __forceinline__ void fetch(frag* regs, const T* base, int64_t stride, int r0, int end,
+                                               int D) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int idx = threadIdx.x + p * kThreads, row = r0 + idx / CH, col = idx % CH * N;
+      regs[p] = chunk(base + row * stride + col, row < end ? D - col : 0);
+    }
+  }
+  static __device__ __forceinline__ frag chunk(const T* p, int cnt) {
+    frag f;
+    if (cnt >= N) {
+      const typename Vec16<T>::utype v = *reinterpret_cast<const typename Vec16<T>::utype*>(p);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = e < cnt ? p[e] : (T)0.f;
+    }
+    return f;
+  }
+  static __device__ __forceinline__ void put(char* lds, const frag* regs) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int idx = threadIdx.x + p * kThreads;
+      *reinterpret_cast<frag*>(lds + at(idx / CH, idx % CH)) = regs[p];
+    }
+  }
+  // A operand whose row is the lane's (row0 + l % 32), step s of a contraction over D
+  static __device__ __forceinline__ frag rows(const char* lds, int row0, int s) {
+    const int lane = threadIdx.x % MN_WAVE;
+    return *reinterpret_cast<const frag*>(lds + at(row0 + lane % 32, 2 * s + lane / 32));
+  }
+  // A operand whose row is column d0 + l % 32 of the tile, step s of a contraction over the 32
+  // rows from row0 on, in the order of an accumulator's registers
+  static __device__ __forceinline__ frag cols(const char* lds, int row0, int s, int d0) {
+    const int lane = threadIdx.x % MN_WAVE, half = lane / 32;
+    frag f;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane % 16, d = d0 + lane % 32 / 16 * 16 + i % 4 * 4;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int row = row0 + 16 * s + 8 * g + 4 * half + i / 4;
+        const char* p = lds + at(row, d / 8) + d % 8 * 2;
+        typedef T quad __attribute__((ext_vector_type(4)));
+        const quad v = __builtin_bit_cast(quad, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * g + e] = v[e];
+      }
+    } else {
+      const int d = d0 + lane % 32;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = row0 + 8 * s + 4 * half + e;
+        f[e] = *reinterpret_cast<const T*>(lds + at(row, d / 4) + d % 4 * 4);
+      }
+    }
+    return f;
+  }
+};
+
+// Steps of a contraction over an accumulator's 32 rows, and the B operand of one of them: the
+// registers in order, rounded to T once (16-bit types: P in [0, 1] and dS carry 2^-8 or 2^-11 of
+// themselves, the rounding the result gets anyway; the sums stay fp32).
+template <typename T>
+struct Acc {
+  static constexpr int N = 16 / (int)sizeof(T);
+  static constexpr int STEPS = 16 / N;
+  static __device__ __forceinline__ typename Mma<T>::frag operand(const f32x16& a, int s) {
+    typename Mma<T>::frag f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = (T)a[s * N + e];
+    return f;
+  }
+};
+
+// Row of an accumulator's register r.
+__device__ __forceinline__ int acc_row(int r) {
+  return r / 4 * 8 + (int)(threadIdx.x % MN_WAVE / 32) * 4 + r % 4;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, MN_WAVE); }
+
+__device__ __forceinline__ bool sees(const Args& a, int i, int j) {
+  return j <= i + a.right && (j >= i - a.left || j < a.sinks);
+}
+
+// Where the keys of queries q0 .. q1 lie: tiles [0, sinks) and [first, last) of ROWS keys.
+struct KeyTiles {
+  int sinks, first, last;
+  __device__ __forceinline__ int count() const { return sinks + last - first; }
+  __device__ __forceinline__ int tile(int n) const { return n < sinks ? n : first + n - sinks; }
+};
+template <int ROWS>
+__device__ __forceinline__ KeyTiles key_tiles(const Args& a, int q0, int q1, int len) {
+  const int lo = max(0, q0 - a.left), hi = min(len - 1, q1 + a.right);
+  KeyTiles t;
+  t.first = lo / ROWS;
+  t.last = hi / ROWS + 1;
+  t.sinks = min((min(a.sinks, len) + ROWS - 1) / ROWS, t.first);
+  return t;
+}
+
+// Does every one of the queries q0 .. q1 see all keys k0 .. k1, does any see any of them?
+__device__ __forceinline__ bool all_visible(const Args& a, int q0, int q1, int k0, int k1, int len) {
+  return k1 < len && k1 <= q0 + a.right && (k0 >= q1 - a.left || k1 < a.sinks);
+}
+__device__ __forceinline__ bool none_visible(const Args& a, int q0, int q1, int k0, int k1) {
+  return k0 > q1 + a.right || (k1 < q0 - a.left && k0 >= a.sinks);
+}
+
+__device__ __forceinline__ int length_of(const Args& a, int b) {
+  if (!a.lengths) return a.T;
+  return min(max(a.lengths[b], 0), a.T);
+}
+
+// B operands of a lane's own row (query or key) straight from memory; `valid` false: zeros.
+template <typename T, int DP>
+__device__ __forceinline__ void own_row(typename Mma<T>::frag* f, const T* row, bool valid, int D) {
+  typedef Tile<T, DP, 64> Ti;
+  const int half = threadIdx.x % MN_WAVE / 32;
+#pragma unroll
+  for (int s = 0; s < Ti::STEPS; ++s) {
+    const int col = (2 * s + half) * Ti::N;
+    f[s] = Ti::chunk(row + col, valid ? D - col : 0);
+  }
+}
+
+// A transposed accumulator (rows = elements of a head, column = the lane's token) to its row,
+// times `factor`; factor 0 (a token behind the end): zeros, whatever was accumulated.
+template <typename T, int DP>
+__device__ __forceinline__ void store_columns(T* row, const f32x16* acc, float factor, int D) {
+  typedef T quad __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  const int half = threadIdx.x % MN_WAVE / 32;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + g * 8 + half * 4;
+      if (d + 4 <= D) {
+        quad v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = factor == 0.f ? (T)0.f : (T)(acc[db][4 * g + e] * factor);
+        *reinterpret_cast<quad*>(row + d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < D) row[d + e] = factor == 0.f ? (T)0.f : (T)(acc[db][4 * g + e] * factor);
+      }
+    }
+}
+
+// Rows of keys in a tile: fp32 rows are twice as long.
+template <typename T>
+constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
+constexpr int kQueries = 32 * kWaves;   // queries (or, for dk / dv, keys) of a workgroup
+
+// --------------------------------------------------------------------------------- forward
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
+  constexpr int R = kRows<T>, KT = R / 32;
+  typedef Tile<T, DP, R> Ti;
+  typedef typename Mma<T>::frag frag;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const uint32_t slot = xcd_slot();
+  const int tile = a.tiles - 1 - (int)(slot % a.tiles);   // long rows of a causal window first
+  const int h = slot / a.tiles % a.Hq, b = slot / a.tiles / a.Hq;
+  const int len = length_of(a, b);
+  const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
+  const int q0 = tile * kQueries, w0 = q0 + wave * 32, i = w0 + lane % 32;
+  T* orow = (T*)a.o + (((int64_t)b * a.T + i) * a.Hq + h) * a.D;
+  float* lse = a.lse + ((int64_t)b * a.Hq + h) * a.T;
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) acc[d] = (f32x16)(0.f);
+  float m = -INFINITY, sum = 0.f;
+  if (q0 < len) {
+    frag qf[Ti::STEPS];
+    own_row<T, DP>(qf, (const T*)a.q + b * a.sq[0] + h * a.sq[2] + i * a.sq[1], i < len, a.D);
+    const T* kb = (const T*)a.k + b * a.sk[0] + h / a.group * a.sk[2];
+    const T* vb = (const T*)a.v + b * a.sv[0] + h / a.group * a.sv[2];
+    const KeyTiles kt = key_tiles<R>(a, q0, min(q0 + kQueries, len) - 1, len);
+    const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
+    frag kreg[Ti::PER], vreg[Ti::PER];
+    Ti::fetch(kreg, kb, a.sk[1], kt.tile(0) * R, len, a.D);
+    Ti::fetch(vreg, vb, a.sv[1], kt.tile(0) * R, len, a.D);
+    for (int n = 0; n < n_tiles; ++n) {
+      char* kl = lds + (n & 1) * 2 * Ti::BYTES;
+      char* vl = kl + Ti::BYTES;
+      Ti::put(kl, kreg);
+      Ti::put(vl, vreg);
+      __syncthreads();   // (the other buffer is written next time, after everyone passed here)
+      if (n + 1 < n_tiles) {
+        Ti::fetch(kreg, kb, a.sk[1], kt.tile(n + 1) * R, len, a.D);
+        Ti::fetch(vreg, vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
+      }
+      const int j0 = kt.tile(n) * R;
+      if (w0 >= len || none_visible(a, w0, w1, j0, j0 + R - 1)) continue;
+      f32x16 s[KT];
+      float top = -INFINITY;
+      const bool whole = all_visible(a, w0, w1, j0, j0 + R - 1, len);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        s[t] = (f32x16)(0.f);
+#pragma unroll
+        for (int st = 0; st < Ti::STEPS; ++st) s[t] = Mma<T>::mul(Ti::rows(kl, t * 32, st), qf[st], s[t]);
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = j0 + t * 32 + acc_row(r);
+            s[t][r] = j < len && sees(a, i, j) ? s[t][r] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+      }
+      top = fmaxf(top, other_half(top)) * a.scale_log2;
+      // a new maximum only where the old one is left behind by more than 2^8: below that P stays
+      // below 2^8 and nothing has to be scaled
+      if (__any(top > m + 8.f)) {
+        const float now = fmaxf(m, top), f = now == -INFINITY ? 1.f : exp2f(m - now);
+        m = now;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+      }
+      const float base = m == -INFINITY ? 0.f : m;   // nothing seen yet: exp2(-inf - 0) = 0
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2, -base));
+          sum += s[t][r];
+        }
+#pragma unroll
+        for (int st = 0; st < Acc<T>::STEPS; ++st) {
+          const frag p = Acc<T>::operand(s[t], st);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+            acc[d] = Mma<T>::mul(Ti::cols(vl, t * 32, st, d * 32), p, acc[d]);
+        }
+      }
+    }
+  }
+  if (i >= a.T) return;
+  sum += other_half(sum);
+  const bool any = i < len && m != -INFINITY;   // (a NaN among the scores: m may be -inf, sum is NaN)
+  const bool valid = i < len && (any || sum != sum);
+  store_columns<T, DP>(orow, acc, valid ? 1.f / sum : 0.f, a.D);
+  if (lane < 32) lse[i] = valid ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
+}
+
+// -------------------------------------------------------------- backward: dq (and rowsum(do o))
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
+  constexpr int R = kRows<T>, KT = R / 32;
+  typedef Tile<T, DP, R> Ti;
+  typedef typename Mma<T>::frag frag;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const uint32_t slot = xcd_slot();
+  const int tile = a.tiles - 1 - (int)(slot % a.tiles);
+  const int h = slot / a.tiles % a.Hq, b = slot / a.tiles / a.Hq;
+  const int len = length_of(a, b);
+  const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
+  const int q0 = tile * kQueries, w0 = q0 + wave * 32, i = w0 + lane % 32;
+  const int64_t row = (((int64_t)b * a.T + i) * a.Hq + h) * a.D;
+  const int64_t stat = ((int64_t)b * a.Hq + h) * a.T + i;
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) acc[d] = (f32x16)(0.f);
+  if (q0 < len) {
+    frag qf[Ti::STEPS], gf[Ti::STEPS];
+    own_row<T, DP>(qf, (const T*)a.out + row, i < len, a.D);
+    own_row<T, DP>(gf, (const T*)a.grad + row, i < len, a.D);
+    float delta = 0.f;
+#pragma unroll
+    for (int s = 0; s < Ti::STEPS; ++s)
+#pragma unroll
+      for (int e = 0; e < Ti::N; ++e) delta += (float)qf[s][e] * (float)gf[s][e];
+    delta += other_half(delta);
+    if (i < len && lane < 32) a.delta[stat] = delta;
+    const float l2 = i < len ? a.lse[stat] * kLog2e : INFINITY;   // no query: P = exp2(-inf) = 0
+    own_row<T, DP>(qf, (const T*)a.q + b * a.sq[0] + h * a.sq[2] + i * a.sq[1], i < len, a.D);
+    const T* kb = (const T*)a.k + b * a.sk[0] + h / a.group * a.sk[2];
+    const T* vb = (const T*)a.v + b * a.sv[0] + h / a.group * a.sv[2];
+    const KeyTiles kt = key_tiles<R>(a, q0, min(q0 + kQueries, len) - 1, len);
+    const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
+    frag kreg[Ti::PER], vreg[Ti::PER];
+    Ti::fetch(kreg, kb, a.sk[1], kt.tile(0) * R, len, a.D);
+    Ti::fetch(vreg, vb, a.sv[1], kt.tile(0) * R, len, a.D);
+    for (int n = 0; n < n_tiles; ++n) {
+      char* kl = lds + (n & 1) * 2 * Ti::BYTES;
+      char* vl = kl + Ti::BYTES;
+      Ti::put(kl, kreg);
+      Ti::put(vl, vreg);
+      __syncthreads();
+      if (n + 1 < n_tiles) {
+        Ti::fetch(kreg, kb, a.sk[1], kt.tile(n + 1) * R, len, a.D);
+        Ti::fetch(vreg, vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
+      }
+      const int j0 = kt.tile(n) * R;
+      if (w0 >= len) continue;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const int jt = j0 + t * 32;
+        if (none_visible(a, w0, w1, jt, jt + 31)) continue;
+        f32x16 s = (f32x16)(0.f), p = (f32x16)(0.f);
+#pragma unroll
+        for (int st = 0; st < Ti::STEPS; ++st) {
+          s = Mma<T>::mul(Ti::rows(kl, t * 32, st), qf[st], s);
+          p = Mma<T>::mul(Ti::rows(vl, t * 32, st), gf[st], p);
+        }
+        const bool whole = all_visible(a, w0, w1, jt, jt + 31, len);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2)) * (p[r] - delta);
+          const int j = jt + acc_row(r);
+          s[r] = whole || (j < len && sees(a, i, j)) ? e : 0.f;
+        }
+#pragma unroll
+        for (int st = 0; st < Acc<T>::STEPS; ++st) {
+          const frag ds = Acc<T>::operand(s, st);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+            acc[d] = Mma<T>::mul(Ti::cols(kl, t * 32, st, d * 32), ds, acc[d]);
+        }
+      }
+    }
+  }
+  if (i < a.T) store_columns<T, DP>((T*)a.dq + row, acc, i < len ? a.scale : 0.f, a.D);
+}
+
+// -------------------------------------------------------------------- backward: dk and dv
+// A wave owns 32 keys (columns) and walks over the queries that see them, for every query head of
+// the group in turn, so a shared head's gradient is one sum in registers, in a fixed order.
+// Key tiles that hold sinks are seen by all later queries: their queries behind the window are
+// given to `nchunks` workgroups more (chunk queries each); all of a split tile's workgroups write
+// fp32 partial results, which attn_join_kernel adds in order.  Without that the one workgroup of
+// the sinks would run T / (left + 128) times as long as any other.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(const Args a) {
+  constexpr int R = kRows<T>, QT = R / 32;
+  typedef Tile<T, DP, R> Ti;
+  typedef typename Mma<T>::frag frag;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int kBuf = 2 * Ti::BYTES + 2 * R * (int)sizeof(float);
+  const uint32_t slot = xcd_slot();
+  const int items = a.tiles + a.sink_tiles * a.nchunks;
+  int item = slot % items;
+  const int hk = slot / items % a.Hkv, b = slot / items / a.Hkv;
+  const int len = length_of(a, b);
+  int tile, part;   // part 0: the window's queries, c + 1: chunk c of those behind it
+  if (item < a.sink_tiles * a.nchunks) {
+    tile = item / a.nchunks;
+    part = item % a.nchunks + 1;
+  } else {
+    tile = item - a.sink_tiles * a.nchunks;
+    part = 0;
+  }
+  const bool split = tile < a.sink_tiles;
+  const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
+  const int k0 = tile * kQueries, w0 = k0 + wave * 32, j = w0 + lane % 32;
+  const int k1 = min(k0 + kQueries, len) - 1, w1 = min(w0 + 31, len - 1);
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = (f32x16)(0.f);
+  // queries of this workgroup
+  int lo = max(0, k0 - a.right), hi = min((int64_t)len - 1, (int64_t)k1 + a.left);
+  if (part > 0) {
+    lo = min((int64_t)a.T, (int64_t)k0 + kQueries + a.left + (int64_t)(part - 1) * a.chunk);
+    hi = min((int64_t)len - 1, (int64_t)lo + a.chunk - 1);
+  } else if (split) {
+    hi = min((int64_t)len - 1, (int64_t)k0 + kQueries - 1 + a.left);
+  } else if (k0 < a.sinks) {
+    hi = len - 1;
+  }
+  if (k0 < len && lo <= hi) {
+    frag kf[Ti::STEPS], vf[Ti::STEPS];
+    own_row<T, DP>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[2] + j * a.sk[1], j < len, a.D);
+    own_row<T, DP>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[2] + j * a.sv[1], j < len, a.D);
+    const int first = lo / R, per_head = hi / R + 1 - first, n_tiles = per_head * a.group;
+    frag qreg[Ti::PER], greg[Ti::PER];
+    float lreg = 0.f, dreg = 0.f;
+    const auto fetch = [&](int n) {
+      const int h = hk * a.group + n / per_head, r0 = (first + n % per_head) * R;
+      Ti::fetch(qreg, (const T*)a.q + b * a.sq[0] + h * a.sq[2], a.sq[1], r0, len, a.D);
+      Ti::fetch(greg, (const T*)a.grad + ((int64_t)b * a.T * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, r0, len,
+                a.D);
+      if (threadIdx.x < R) {
+        const int i = r0 + threadIdx.x;
+        const int64_t stat = ((int64_t)b * a.Hq + h) * a.T + i;
+        lreg = i < len ? a.lse[stat] * kLog2e : INFINITY;
+        dreg = i < len ? a.delta[stat] : 0.f;
+      }
+    };
+    fetch(0);
+    for (int n = 0; n < n_tiles; ++n) {
+      char* ql = lds + (n & 1) * kBuf;
+      char* gl = ql + Ti::BYTES;
+      float* ll = reinterpret_cast<float*>(gl + Ti::BYTES);
+      float* dl = ll + R;
+      Ti::put(ql, qreg);
+      Ti::put(gl, greg);
+      if (threadIdx.x < R) {
+        ll[threadIdx.x] = lreg;
+        dl[threadIdx.x] = dreg;
+      }
+      __syncthreads();
+      if (n + 1 < n_tiles) fetch(n + 1);
+      const int i0 = (first + n % per_head) * R;
+      if (w0 >= len) continue;
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const int it = i0 + t * 32;
+        // (queries outside [lo, hi] belong to another workgroup of the tile)
+        if (it > hi || it + 31 < lo || none_visible(a, it, it + 31, w0, w1)) continue;
+        f32x16 s = (f32x16)(0.f), p = (f32x16)(0.f);
+#pragma unroll
+        for (int st = 0; st < Ti::STEPS; ++st) {
+          s = Mma<T>::mul(Ti::rows(ql, t * 32, st), kf[st], s);
+          p = Mma<T>::mul(Ti::rows(gl, t * 32, st), vf[st], p);
+        }
+        const bool whole = it >= lo && it + 31 <= hi && all_visible(a, it, it + 31, w0, w0 + 31, len);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4_t l2 = *reinterpret_cast<const float4_t*>(ll + t * 32 + g * 8 + lane / 32 * 4);
+          const float4_t de = *reinterpret_cast<const float4_t*>(dl + t * 32 + g * 8 + lane / 32 * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e, i = it + acc_row(r);
+            float pe = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2[e]));
+            const float ds = pe * (p[r] - de[e]);
+            const bool see = whole || (i >= lo && i <= hi && j < len && sees(a, i, j));
+            s[r] = see ? pe : 0.f;
+            p[r] = see ? ds : 0.f;
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < Acc<T>::STEPS; ++st) {
+          const frag pf = Acc<T>::operand(s, st), df = Acc<T>::operand(p, st);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            dv[d] = Mma<T>::mul(Ti::cols(gl, t * 32, st, d * 32), pf, dv[d]);
+            dk[d] = Mma<T>::mul(Ti::cols(ql, t * 32, st, d * 32), df, dk[d]);
+          }
+        }
+      }
+    }
+  }
+  if (j >= a.T) return;
+  if (split) {
+    // [b, hk, tile, part, dk / dv, key, D]
+    float* out = a.parts + (((((int64_t)b * a.Hkv + hk) * a.sink_tiles + tile) * (a.nchunks + 1) + part) * 2 *
+                                kQueries + (j - k0)) * a.D;
+    store_columns<float, DP>(out, dk, a.scale, a.D);
+    store_columns<float, DP>(out + (int64_t)kQueries * a.D, dv, 1.f, a.D);
+  } else {
+    const int64_t row = (((int64_t)b * a.T + j) * a.Hkv + hk) * a.D;
+    store_columns<T, DP>((T*)a.dk + row, dk, j < len ? a.scale : 0.f, a.D);
+    store_columns<T, DP>((T*)a.dv + row, dv, j < len ? 1.f : 0.f, a.D);
+  }
+}
+
+// Adds the partial results of the split key tiles in order: one thread per element.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(const Args a, int64_t total) {
+  const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (e >= total) return;
+  const int64_t per_tile = (int64_t)kQueries * a.D;
+  const int64_t in_tile = e % per_tile, which = e / per_tile % 2, tile = e / per_tile / 2 % a.sink_tiles;
+  const int64_t bh = e / per_tile / 2 / a.sink_tiles;
+  const int64_t j = tile * kQueries + in_tile / a.D, b = bh / a.Hkv, hk = bh % a.Hkv;
+  if (j >= a.T) return;
+  const float* p = a.parts + ((bh * a.sink_tiles + tile) * (a.nchunks + 1) * 2 + which) * per_tile + in_tile;
+  float s = 0.f;
+  if (j < length_of(a, (int)b))
+    for (int c = 0; c <= a.nchunks; ++c) s += p[(int64_t)c * 2 * per_tile];
+  T* out = (T*)(which ? a.dv : a.dk);
+  out[((b * a.T + j) * a.Hkv + hk) * a.D + in_tile % a.D] = (T)s;
+}
+
+// ------------------------------------------------------------------------------- host side
+int check(const mn_attention* d) {
+  if (!d || d->B < 0 || d->T < 0 || d->Hq <= 0 || d->Hkv <= 0 || d->D <= 0) return MN_EINVAL;
+  if (d->Hq % d->Hkv || d->left < -1 || d->right < -1 || d->sinks < 0) return MN_EINVAL;
+  if (!(d->scale > 0.f) || d->scale > 1e30f) return MN_EINVAL;
+  if (d->D > kMaxD || d->T >= (1 << 28)) return MN_EUNSUPPORTED;
+  // one workgroup per tile, head and entry, counted in 32 bits (dk / dv: at most twice the tiles)
+  const int64_t tiles = (d->T + kQueries - 1) / kQueries;
+  if (d->B >= (1 << 28) || d->Hq >= (1 << 20) || (tiles && d->B * d->Hq > (1ll << 30) / tiles))
+    return MN_EUNSUPPORTED;
+  return MN_OK;
+}
+
+// "No limit" and limits beyond the sequence are T: sums with them stay inside 32 bits.
+int32_t limit(int64_t v, int64_t T) { return (int32_t)(v < 0 || v > T ? T : v); }
+
+// How the queries behind the window of the key tiles with sinks are cut.  A chunk is as long as
+// the window a plain tile walks over, but at most 32 of them; not cut where the sinks are more
+// than an eighth of the keys (enough workgroups share the long walk then).
+void split_for(const mn_attention* d, Args* a) {
+  a->sink_tiles = a->nchunks = 0;
+  a->chunk = 1;
+  const int64_t T = d->T, left = limit(d->left, T);
+  const int64_t sinks = d->sinks < T ? d->sinks : T, tiles = (sinks + kQueries - 1) / kQueries;
+  const int64_t behind = T - kQueries - left;   // queries behind the window of the first tile
+  if (sinks == 0 || behind <= 0 || tiles * kQueries * 8 > T) return;
+  int64_t chunk = kQueries + left;
+  if (chunk < (behind + 31) / 32) chunk = (behind + 31) / 32;
+  chunk = (chunk + 63) / 64 * 64;
+  a->sink_tiles = (int32_t)tiles;
+  a->chunk = (int32_t)chunk;
+  a->nchunks = (int32_t)((behind + chunk - 1) / chunk);
+}
+
+size_t parts_floats(const mn_attention* d, const Args& a) {
+  return (size_t)d->B * d->Hkv * a.sink_tiles * (a.nchunks + 1) * 2 * kQueries * d->D;
+}
+
+Args args_for(const mn_attention* d) {
+  Args a = {};
+  for (int k = 0; k < 3; ++k) {
+    a.sq[k] = d->q_stride[k];
+    a.sk[k] = d->k_stride[k];
+    a.sv[k] = d->v_stride[k];
+  }
+  a.T = (int32_t)d->T; a.Hq = d->Hq; a.Hkv = d->Hkv; a.D = d->D;
+  a.left = limit(d->left, d->T); a.right = limit(d->right, d->T);
+  a.sinks = (int32_t)(d->sinks < d->T ? d->sinks : d->T);
+  a.tiles = (int32_t)((d->T + kQueries - 1) / kQueries);
+  a.group = d->Hq / d->Hkv;
+  a.scale = d->scale;
+  a.scale_log2 = d->scale * kLog2e;
+  return a;
+}
+
+// f(head size rounded up to 32) as a constant
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+template <typename F>
+int for_width(int D, F f) {
+  if (D <= 32) return f(Int<32>());
+  if (D <= 64) return f(Int<64>());
+  if (D <= 96) return f(Int<96>());
+  return f(Int<128>());
+}
+
+// Dynamic LDS of more than 64 KB has to be asked for, once per kernel and device.
+template <typename K>
+bool raise_lds(K kernel, int bytes) {
+  return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+}
+
+template <typename T, int DP>
+constexpr int kLdsQ = 4 * Tile<T, DP, kRows<T>>::BYTES;   // two buffers of two tiles
+template <typename T, int DP>
+constexpr int kLdsKv = kLdsQ<T, DP> + 4 * kRows<T> * (int)sizeof(float);   // and two rows' statistics
+
+template <typename T, int DP>
+bool init_one() {
+  return raise_lds(attn_fwd_kernel<T, DP>, kLdsQ<T, DP>) && raise_lds(attn_dq_kernel<T, DP>, kLdsQ<T, DP>) &&
+         raise_lds(attn_dkv_kernel<T, DP>, kLdsKv<T, DP>);
+}
+template <typename T>
+bool init_type() {
+  return init_one<T, 32>() && init_one<T, 64>() && init_one<T, 96>() && init_one<T, 128>();
+}
+
+}  // namespace
+
+// The limits of dynamic LDS, which are not a stream operation: from mn_init, and again from the
+// entry points (a caller that never calls mn_init).
+bool mn_attention_init() { return init_type<float>() && init_type<bf16_t>() && init_type<f16_t>(); }
+
+extern "C" {
+
+int mn_attention_fwd(const mn_attention* d, const void* q, const void* k, const void* v, const int32_t* lengths,
+                     void* out, float* lse, int dtype, mn_stream_t stream) {
+  const int st = check(d);
+  if (st != MN_OK) return st;
+  return mn_for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (d->B == 0 || d->T == 0) return (int)MN_OK;
+    if (!q || !k || !v || !out || !lse) return (int)MN_EINVAL;
+    Args a = args_for(d);
+    a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse; a.lengths = lengths;
+    const unsigned grid = (unsigned)(a.tiles * d->Hq * d->B);
+    return for_width(d->D, [&](auto w) {
+      constexpr int DP = decltype(w)::value, lds = kLdsQ<T, DP>;
+      if (!raise_lds(attn_fwd_kernel<T, DP>, lds)) return (int)MN_ELAUNCH;
+      attn_fwd_kernel<T, DP><<<grid, kThreads, lds, mn_stream(stream)>>>(a);
+      return mn_launch_status();
+    });
+  });
+}
+
+size_t mn_attention_bwd_ws_bytes(const mn_attention* d) {
+  if (check(d) != MN_OK) return 0;
+  Args a = {};
+  split_for(d, &a);
+  return ((size_t)d->B * d->Hq * d->T + parts_floats(d, a)) * sizeof(float);
+}
+
+int mn_attention_bwd(const mn_attention* d, const void* grad, const void* q, const void* k, const void* v,
+                     const void* out, const float* lse, const int32_t* lengths, void* dq, void* dk, void* dv,
+                     int dtype, void* ws, size_t ws_bytes, mn_stream_t stream) {
+  const int st = check(d);
+  if (st != MN_OK) return st;
+  return mn_for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (d->B == 0 || d->T == 0) return (int)MN_OK;
+    if (!grad || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return (int)MN_EINVAL;
+    if (!ws || ws_bytes < mn_attention_bwd_ws_bytes(d) || !mn_aligned(ws, 4)) return (int)MN_EINVAL;
+    Args a = args_for(d);
+    a.q = q; a.k = k; a.v = v; a.out = out; a.grad = grad; a.lse = const_cast<float*>(lse);
+    a.dq = dq; a.dk = dk; a.dv = dv; a.lengths = lengths;
+    a.delta = (float*)ws;
+    a.parts = a.delta + (size_t)d->B * d->Hq * d->T;
+    split_for(d, &a);
+    hipStream_t s = mn_stream(stream);
+    const int rc = for_width(d->D, [&](auto w) {
+      constexpr int DP = decltype(w)::value, lds_q = kLdsQ<T, DP>, lds_kv = kLdsKv<T, DP>;
+      if (!raise_lds(attn_dq_kernel<T, DP>, lds_q) || !raise_lds(attn_dkv_kernel<T, DP>, lds_kv))
+        return (int)MN_ELAUNCH;
+      attn_dq_kernel<T, DP><<<(unsigned)(a.tiles * d->Hq * d->B), kThreads, lds_q, s>>>(a);
+      const unsigned items = (unsigned)(a.tiles + a.sink_tiles * a.nchunks);
+      attn_dkv_kernel<T, DP><<<(unsigned)(items * d->Hkv * d->B), kThreads, lds_kv, s>>>(a);
+      return mn_launch_status();
+    });
+    if (rc != MN_OK || !a.sink_tiles) return rc;
+    const int64_t total = d->B * d->Hkv * a.sink_tiles * 2 * kQueries * d->D;
+    attn_join_kernel<T><<<(unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, total);
+    return mn_launch_status();
+  });
+}
+
+}  // extern "C"

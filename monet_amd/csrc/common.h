@@ -39,10 +39,12 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// Per-device set-up that is not a stream operation (see mn_init); defined in bn.hip and
-// conv_wino.hip.  Both are idempotent and also run lazily from the entry points that need them.
+// Per-device set-up that is not a stream operation (see mn_init); defined in bn.hip,
+// conv_wino.hip and attention.hip.  All are idempotent and also run lazily from the entry points
+// that need them.
 bool mn_bn_static_init();
 bool mn_wino_init();
+bool mn_attention_init();
 
 // Workgroups are handed to the 8 XCDs (each with its own L2) round-robin in launch order.
 // xcd_slot() turns a workgroup's launch index into a position in a LOGICAL order in which each

@@ -95,6 +95,56 @@ def test_rotary_refusals():
         assert call(**empty) == _lib.MN_OK, empty
 
 
+def _attention(**kw):
+    d = _lib.AttentionDesc(B=2, T=300, Hq=4, Hkv=2, D=64, left=10, right=0, sinks=1, scale=0.125)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_attention_refusals():
+    f, b, size = lib().mn_attention_fwd, lib().mn_attention_bwd, lib().mn_attention_bwd_ws_bytes
+
+    def fwd(q=P, k=P, v=P, out=P, lse=P, dtype=F32, **kw):
+        return f(ctypes.byref(_attention(**kw)), q, k, v, None, out, lse, dtype, None)
+
+    assert f(None, P, P, P, None, P, P, F32, None) == _lib.MN_EINVAL and size(None) == 0
+    for bad in (dict(B=-1), dict(T=-1), dict(Hq=0), dict(Hkv=0), dict(D=0), dict(Hq=5), dict(left=-2),
+                dict(right=-2), dict(sinks=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                dict(scale=float("inf")), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
+                dict(lse=None)):
+        assert fwd(**bad) == _lib.MN_EINVAL, bad
+    for bad in (dict(D=129), dict(T=1 << 28), dict(B=1 << 28), dict(Hq=1 << 20, Hkv=1 << 20),
+                dict(B=1 << 20, T=1 << 20), dict(dtype=5)):
+        assert fwd(**bad) == _lib.MN_EUNSUPPORTED, bad
+    for empty in (dict(B=0), dict(T=0)):
+        assert fwd(**empty) == _lib.MN_OK, empty
+
+    def bwd(hole=None, ws=P, nbytes=None, **kw):
+        d = _attention(**kw)
+        ptrs = [None if k == hole else P for k in range(10)]
+        return b(ctypes.byref(d), *ptrs, F32, ws, size(ctypes.byref(d)) if nbytes is None else nbytes, None)
+
+    for hole in (0, 1, 2, 3, 4, 5, 7, 8, 9):       # 6 is `lengths`, which may be missing
+        assert bwd(hole) == _lib.MN_EINVAL, hole
+    assert bwd(ws=None) == _lib.MN_EINVAL and bwd(ws=P + 2) == _lib.MN_EINVAL and bwd(nbytes=8) == _lib.MN_EINVAL
+    assert bwd(D=129, nbytes=1 << 40) == _lib.MN_EUNSUPPORTED
+
+
+def test_attention_workspace():
+    size = lambda **kw: lib().mn_attention_bwd_ws_bytes(ctypes.byref(_attention(**kw)))
+    rows = 4 * 2 * 4          # fp32 per token: batch 2, 4 heads
+    assert size() == rows * 300 and size(sinks=0) == rows * 300 and size(left=-1, T=5000) == rows * 5000
+    assert size(T=0) == 0 and size(D=129) == 0
+    # sinks behind a window: partial results of at most 33 workgroups per tile of 128 keys
+    for T, left, sinks in ((1100, 60, 1), (15808, 1024, 4), (1 << 20, 0, 200), (40000, 128, 4000)):
+        parts = size(T=T, left=left, sinks=sinks) - rows * T
+        tile = 2 * 2 * 2 * 128 * 64 * 4   # batch, key heads, dk and dv
+        tiles = (sinks + 127) // 128
+        assert parts % (tile * tiles) == 0 and 2 <= parts // (tile * tiles) <= 33, (T, left, sinks)
+    assert size(T=2000, left=10, sinks=300) == rows * 2000   # more than an eighth of the keys
+
+
 def test_operators_refuse_cpu_tensors():
     x = torch.zeros(2, 4)
     with pytest.raises(RuntimeError, match="GPU tensor"):
@@ -107,6 +157,8 @@ def test_operators_refuse_cpu_tensors():
         lm_ops.dropout.dropout_state("cpu")
     with pytest.raises(RuntimeError, match="GPU tensor"):
         lm_ops.rotary.rotary_forward(x[None, None], torch.zeros(1, 2), (2,))
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        lm_ops.attention.window_attention_forward(x[None, None], x[None, None], x[None, None])
 
 
 def test_registered_in_every_solver_mode():
@@ -114,7 +166,8 @@ def test_registered_in_every_solver_mode():
                  "conv_normal"):
         for name, cls in (("aten::layer_norm", lm_ops.layernorm.InputActLayerNorm),
                           ("monet::dropout", lm_ops.dropout.CounterDropout),
-                          ("monet::rotary", lm_ops.rotary.Rotary)):
+                          ("monet::rotary", lm_ops.rotary.Rotary),
+                          ("monet::window_attention", lm_ops.attention.WindowAttention)):
             assert lm_ops.list_ops(mode, name) == [cls]
         # the operator that replays torch's own dropout stays what it was
         assert lm_ops.list_ops(mode, "aten::dropout") == [lm_ops.elementary.Dropout]
