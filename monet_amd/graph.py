@@ -281,7 +281,7 @@ class Graph:
                 const[n.output().unique()] = n.output().toIValue()
             elif kind in ('prim::ListConstruct', 'prim::TupleConstruct'):
                 lists[n.output().unique()] = [i.unique() for i in n.inputs()]
-            elif kind.startswith('aten::'):
+            elif kind.startswith(('aten::', 'monet::')):
                 out = n.output()
                 connected = out.unique() in tracked
                 if not connected and len(out.uses()) == 0:
@@ -319,7 +319,7 @@ class Graph:
                 print('Unknown OP', kind, n)
 
         for o in trace.outputs():
-            if o.node().kind().startswith('aten::'):
+            if o.node().kind().startswith(('aten::', 'monet::')):
                 g._outputs.append(node_of[o.unique()])
             elif o.node().kind() == 'prim::TupleConstruct':
                 for i in o.node().inputs():

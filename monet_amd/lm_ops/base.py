@@ -58,6 +58,10 @@ class OP:
     # ReLU backward does, lrrelu.cpp:14-15).  The executor hands such an operator a private
     # copy when another pending gradient still shares that storage.
     overwrites_grad = False
+    # True: a forward that is run again within a step has to find the `params` its first run left
+    # (the executor restores them, and clears them between steps).  BatchNorm's operators are
+    # known by name.
+    recompute_needs_params = False
 
     def intermediate(self, *args, **kwargs):
         return None

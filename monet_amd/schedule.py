@@ -77,7 +77,7 @@ class Schedule(Graph):
                     self.deltensors[j].append(si.solver_to_graph[i])
 
         self._plan = []        # per timestep: list of instructions
-        self._ops0 = []        # batch-norm operators of the forward pass (state reset per step)
+        self._ops0 = []        # operators of the forward pass whose state lasts one step
         self._regs = [None] * self.lennodes
         self._ints = [None] * self.lennodes
         self._state = [None] * self.lennodes
@@ -198,13 +198,13 @@ class Schedule(Graph):
                                 "nor recomputed" % (t, n.op, k, a.index)
                     args = tuple((False, a.value) if isinstance(a, ComputeNode.V)
                                  else (True, (a.index, a.requires_grad)) for a in n.args)
-                    is_bn = is_batch_norm(n.op)
-                    if is_bn and t == 0:
+                    keeps = is_batch_norm(n.op) or op.recompute_needs_params
+                    if keeps and t == 0:
                         self._ops0.append(op)
                     inplace_src = -1
                     if getattr(op, 'inplace', False):
                         inplace_src = n.args[0].index  # the tensor the kernel overwrites
-                    plan.append((_FWD, op, k, args, with_int, is_bn and t > 0,
+                    plan.append((_FWD, op, k, args, with_int, keeps and t > 0,
                                  hasattr(op, 'params'), isinstance(op, lm_ops.NativeOP), inplace_src))
                     live.add(k)
                     if with_int:
@@ -363,7 +363,7 @@ class Schedule(Graph):
             "expected %d inputs and parameters, got %d" % (len(self._leaves), len(args))
         self._args = args
         for op in self._ops0:
-            op.params = None  # fresh batch statistics every step
+            op.params = None  # fresh batch statistics and dropout states every step
         regs = self._regs
         for k in self._leaves:
             regs[k] = args[k]

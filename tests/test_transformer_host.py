@@ -171,3 +171,60 @@ def test_registered_in_every_solver_mode():
             assert lm_ops.list_ops(mode, name) == [cls]
         # the operator that replays torch's own dropout stays what it was
         assert lm_ops.list_ops(mode, "aten::dropout") == [lm_ops.elementary.Dropout]
+
+
+# ------------------------------------------------------------------ traced, solved, compiled
+def _traced():
+    from transformer_net import PATCH, TOKENS, PatchNet
+    from monet_amd.graph import Graph
+    torch.manual_seed(0)
+    return Graph.create(PatchNet(), (TOKENS, PATCH))
+
+
+def test_a_traced_model_names_the_operators():
+    g = _traced()
+    ops = [n.op for n in g.nodes if hasattr(n, "op")]
+    assert ops.count("monet::rotary") == 4 and ops.count("monet::window_attention") == 2
+    assert ops.count("monet::dropout") == 4 and ops.count("aten::layer_norm") == 5
+    from transformer_net import TOKENS
+    for n in g.nodes:
+        if getattr(n, "op", "") == "monet::window_attention":
+            assert n.shape == [-1, TOKENS, 4, 12] and n.has_backward
+            assert [a.value for a in n.args[3:]] == [None, 13, 2, 1, None]
+
+
+def test_outside_a_trace_cpu_tensors_are_refused():
+    from monet_amd import functional as MF
+    x = torch.zeros(1, 2, 2, 8)
+    for call in (lambda: MF.dropout(x, 0.5), lambda: MF.window_attention(x, x, x),
+                 lambda: MF.rotary(x, torch.zeros(1, 2), (2,))):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
+    assert MF.dropout(x, 0.5, training=False) is x and MF.dropout(x, 0.0) is x
+    with pytest.raises(RuntimeError, match="between 0 and 1"):
+        MF.dropout(x, 1.5)
+
+
+@pytest.mark.parametrize("mode", ["normal", "multiway_newnode", "inplace_conv_multiway_newnode"])
+def test_schedules_of_a_traced_model_compile(mode):
+    """The solver's plan, generous and tight, compiles; dropouts that run again in the backward are
+    marked to find the state of their first run."""
+    from monet_amd.schedule import Schedule, _FWD
+    from monet_amd.solver import Model
+    from monet_amd.solver_info import SolverInfo
+    from transformer_net import cheap_dropout_cost
+    g = _traced()
+    si = SolverInfo(16, "patch", mode)
+    si.extract(g, cost_fn=cheap_dropout_cost(si))
+    total = sum(n.mem for i, n in si.nodes.items() if i < si.loss) + si.nodes[si.loss].fixed_mem
+    again = 0
+    for frac in (1.5, 0.55, 0.45):
+        sol = Model(si, frac * total / 2 ** 30, time_limit=60, mip_rel_gap=0.1).solve()
+        sched = Schedule(g, si)
+        sched.init_schedule(sol, si.mode)
+        for t, plan in enumerate(sched._plan):
+            for ins in plan:
+                if ins[0] == _FWD and type(ins[1]).__name__ == "CounterDropout":
+                    assert ins[5] == (t > 0)
+                    again += t > 0
+    assert again > 0
