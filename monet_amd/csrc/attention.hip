@@ -45,7 +45,8 @@ struct Args {
   int64_t sq[3], sk[3], sv[3];          // strides of b, t, h in elements
   int32_t T, Hq, Hkv, D, left, right, sinks;
   int32_t tiles, group;
-  int32_t sink_tiles, chunk, nchunks;   // dk / dv: see there
+  int32_t sink_tiles, sink_rows, chunk, nchunks;   // dk / dv: see there
+  int32_t fold;                         // tiles differ in work: see tile_of
   float scale, scale_log2;
 };
 
@@ -76,6 +77,25 @@ struct Mma<float> {   // four contraction slots a lane: four instructions of two
   }
 };
 
+// 16 bytes a lane from memory to LDS (wave-uniform address `lds` + 16 * lane), asynchronous: the
+// data is there after wait_loads() and a barrier.  In assembly because the compiler, which cannot
+// tell the two buffers apart, would wait for the load before the next read of LDS; m0 is put back.
+__device__ __forceinline__ void load_to_lds(const void* p, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+               "s_mov_b32 m0, %0"
+               : "=&s"(m0)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p)
+               : "memory");
+}
+// Keeps the scheduler from sinking loads to their uses: several LDS reads are in flight while
+// earlier ones are multiplied.
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
 // One tile of rows in LDS: DP elements a row (D rounded up to 32, zeros behind D).
 template <typename T, int DP, int ROWS>
 struct Tile {
@@ -86,7 +106,7 @@ struct Tile {
   static constexpr int STEPS = CH / 2;               // steps of a contraction over D
   static constexpr int BYTES = ROWS * NC * 16;
   static constexpr int PER = ROWS * CH / kThreads;   // chunks a thread stages
-  static_assert(ROWS * CH % kThreads == 0, "whole chunks per thread");
+  static_assert(ROWS * CH % kThreads == 0 && ROWS * NC % kThreads == 0, "whole chunks per thread");
 
   static __device__ __forceinline__ int swz(int row) {
     if (NC >= 16) return (row & 3) << 2 | (row >> 2 & 3);
@@ -125,6 +145,27 @@ struct Tile {
       *reinterpret_cast<frag*>(lds + at(idx / CH, idx % CH)) = regs[p];
     }
   }
+  // global -> LDS without registers: the memory system writes 16 bytes per lane, 1 KB per wave and
+  // instruction in the order of the lanes, so the swizzle is in which chunk a lane asks for.
+  // Rows from `end` on repeat the last one: what is multiplied with them is zero.  Needs
+  // 16-byte aligned rows of whole chunks; chunks behind D are not written (see clear).
+  static __device__ __forceinline__ void load(uint32_t lds, const T* base, int64_t stride, int r0, int end,
+                                              int D) {
+#pragma unroll
+    for (int p = 0; p < ROWS * NC / kThreads; ++p) {
+      const int slot = threadIdx.x + p * kThreads, row = slot / NC, chunk = slot % NC ^ swz(row);
+      const uint32_t at = lds + (p * kThreads + (threadIdx.x & ~(MN_WAVE - 1))) * 16;
+      if (chunk * N < D) load_to_lds(base + min(r0 + row, end - 1) * stride + chunk * N, at);
+    }
+  }
+  static __device__ __forceinline__ void clear(char* lds, int D) {
+    if (D == NC * N) return;
+#pragma unroll
+    for (int p = 0; p < ROWS * NC / kThreads; ++p) {
+      const int slot = threadIdx.x + p * kThreads, row = slot / NC, chunk = slot % NC ^ swz(row);
+      if (chunk * N >= D) *reinterpret_cast<frag*>(lds + slot * 16) = (frag)(0.f);
+    }
+  }
   // A operand whose row is the lane's (row0 + l % 32), step s of a contraction over D
   static __device__ __forceinline__ frag rows(const char* lds, int row0, int s) {
     const int lane = threadIdx.x % MN_WAVE;
@@ -158,6 +199,46 @@ struct Tile {
   }
 };
 
+// Two buffers of two tiles (keys and values, or queries and gradients): while one is multiplied,
+// the other is filled, straight from memory if DIRECT, through registers otherwise.
+template <typename T, int DP, int ROWS, bool DIRECT, int EXTRA>
+struct Stage {
+  typedef Tile<T, DP, ROWS> Ti;
+  static constexpr int kBuf = 2 * Ti::BYTES + EXTRA;
+  char* lds;
+  typename Ti::frag r0[DIRECT ? 1 : Ti::PER], r1[DIRECT ? 1 : Ti::PER];
+
+  __device__ __forceinline__ char* buffer(int n) const { return lds + (n & 1) * kBuf; }
+  __device__ __forceinline__ void init(char* p, int D) {
+    lds = p;
+    if (DIRECT)
+      for (int n = 0; n < 2; ++n) {
+        Ti::clear(buffer(n), D);
+        Ti::clear(buffer(n) + Ti::BYTES, D);
+      }
+  }
+  // tile n: rows row0 .. of two heads
+  __device__ __forceinline__ void begin(int n, const T* a, int64_t sa, const T* b, int64_t sb, int row0,
+                                        int end, int D) {
+    if constexpr (DIRECT) {
+      const uint32_t at = lds_address(buffer(n));
+      Ti::load(at, a, sa, row0, end, D);
+      Ti::load(at + Ti::BYTES, b, sb, row0, end, D);
+    } else {
+      Ti::fetch(r0, a, sa, row0, end, D);
+      Ti::fetch(r1, b, sb, row0, end, D);
+    }
+  }
+  __device__ __forceinline__ void finish(int n) {
+    if constexpr (DIRECT) {
+      wait_loads();
+    } else {
+      Ti::put(buffer(n), r0);
+      Ti::put(buffer(n) + Ti::BYTES, r1);
+    }
+  }
+};
+
 // Steps of a contraction over an accumulator's 32 rows, and the B operand of one of them: the
 // registers in order, rounded to T once (16-bit types: P in [0, 1] and dS carry 2^-8 or 2^-11 of
 // themselves, the rounding the result gets anyway; the sums stay fp32).
@@ -179,6 +260,9 @@ __device__ __forceinline__ int acc_row(int r) {
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, MN_WAVE); }
+
+// In a branch few tiles take: keeps the compiler from computing both sides for all of them.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 __device__ __forceinline__ bool sees(const Args& a, int i, int j) {
   return j <= i + a.right && (j >= i - a.left || j < a.sinks);
@@ -249,21 +333,40 @@ __device__ __forceinline__ void store_columns(T* row, const f32x16* acc, float f
     }
 }
 
+// Which tile of which head (counting the batch) a workgroup has.  Each of the 8 XCDs runs a
+// contiguous range of (head, tile), so that neighbours find each other's keys in its L2.  Where
+// tiles differ in work (one side of the window open), a head's tiles are taken in pairs from both
+// ends, which gives any range the same share of long and short ones, and a range runs its long
+// ones first.
+struct TileOf {
+  int tile, head;
+};
+__device__ __forceinline__ TileOf tile_of(const Args& a, int tiles, bool last_is_long) {
+  if (!a.fold) {
+    const uint32_t slot = xcd_slot();
+    return {(int)(slot % tiles), (int)(slot / tiles)};
+  }
+  const uint32_t total = gridDim.x, xcd = blockIdx.x & 7u, j = blockIdx.x >> 3, rem = total & 7u;
+  const uint32_t start = xcd * (total >> 3) + (xcd < rem ? xcd : rem), n = (total >> 3) + (xcd < rem ? 1 : 0);
+  const uint32_t half = (n + 1) / 2, slot = start + (j < half ? 2 * j : 2 * (j - half) + 1);
+  const int k = slot % tiles, from_front = k & 1 ? tiles - 1 - k / 2 : k / 2;
+  return {last_is_long ? tiles - 1 - from_front : from_front, (int)(slot / tiles)};
+}
+
 // Rows of keys in a tile: fp32 rows are twice as long.
 template <typename T>
 constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
 constexpr int kQueries = 32 * kWaves;   // queries (or, for dk / dv, keys) of a workgroup
 
 // --------------------------------------------------------------------------------- forward
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
   constexpr int R = kRows<T>, KT = R / 32;
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const uint32_t slot = xcd_slot();
-  const int tile = a.tiles - 1 - (int)(slot % a.tiles);   // long rows of a causal window first
-  const int h = slot / a.tiles % a.Hq, b = slot / a.tiles / a.Hq;
+  const TileOf me = tile_of(a, a.tiles, a.left > a.right);
+  const int tile = me.tile, h = me.head % a.Hq, b = me.head / a.Hq;
   const int len = length_of(a, b);
   const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
   const int q0 = tile * kQueries, w0 = q0 + wave * 32, i = w0 + lane % 32;
@@ -280,19 +383,15 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
     const T* vb = (const T*)a.v + b * a.sv[0] + h / a.group * a.sv[2];
     const KeyTiles kt = key_tiles<R>(a, q0, min(q0 + kQueries, len) - 1, len);
     const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
-    frag kreg[Ti::PER], vreg[Ti::PER];
-    Ti::fetch(kreg, kb, a.sk[1], kt.tile(0) * R, len, a.D);
-    Ti::fetch(vreg, vb, a.sv[1], kt.tile(0) * R, len, a.D);
+    Stage<T, DP, R, DIRECT, 0> stage;
+    stage.init(lds, a.D);
+    stage.begin(0, kb, a.sk[1], vb, a.sv[1], kt.tile(0) * R, len, a.D);
     for (int n = 0; n < n_tiles; ++n) {
-      char* kl = lds + (n & 1) * 2 * Ti::BYTES;
-      char* vl = kl + Ti::BYTES;
-      Ti::put(kl, kreg);
-      Ti::put(vl, vreg);
-      __syncthreads();   // (the other buffer is written next time, after everyone passed here)
-      if (n + 1 < n_tiles) {
-        Ti::fetch(kreg, kb, a.sk[1], kt.tile(n + 1) * R, len, a.D);
-        Ti::fetch(vreg, vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
-      }
+      const char* kl = stage.buffer(n);
+      const char* vl = kl + Ti::BYTES;
+      stage.finish(n);
+      __syncthreads();   // (everyone is done with the other buffer)
+      if (n + 1 < n_tiles) stage.begin(n + 1, kb, a.sk[1], vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
       const int j0 = kt.tile(n) * R;
       if (w0 >= len || none_visible(a, w0, w1, j0, j0 + R - 1)) continue;
       f32x16 s[KT];
@@ -304,6 +403,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
 #pragma unroll
         for (int st = 0; st < Ti::STEPS; ++st) s[t] = Mma<T>::mul(Ti::rows(kl, t * 32, st), qf[st], s[t]);
         if (!whole) {
+          keep_branch();
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int j = j0 + t * 32 + acc_row(r);
@@ -352,15 +452,14 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
 }
 
 // -------------------------------------------------------------- backward: dq (and rowsum(do o))
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
   constexpr int R = kRows<T>, KT = R / 32;
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const uint32_t slot = xcd_slot();
-  const int tile = a.tiles - 1 - (int)(slot % a.tiles);
-  const int h = slot / a.tiles % a.Hq, b = slot / a.tiles / a.Hq;
+  const TileOf me = tile_of(a, a.tiles, a.left > a.right);
+  const int tile = me.tile, h = me.head % a.Hq, b = me.head / a.Hq;
   const int len = length_of(a, b);
   const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
   const int q0 = tile * kQueries, w0 = q0 + wave * 32, i = w0 + lane % 32;
@@ -386,19 +485,15 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
     const T* vb = (const T*)a.v + b * a.sv[0] + h / a.group * a.sv[2];
     const KeyTiles kt = key_tiles<R>(a, q0, min(q0 + kQueries, len) - 1, len);
     const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
-    frag kreg[Ti::PER], vreg[Ti::PER];
-    Ti::fetch(kreg, kb, a.sk[1], kt.tile(0) * R, len, a.D);
-    Ti::fetch(vreg, vb, a.sv[1], kt.tile(0) * R, len, a.D);
+    Stage<T, DP, R, DIRECT, 0> stage;
+    stage.init(lds, a.D);
+    stage.begin(0, kb, a.sk[1], vb, a.sv[1], kt.tile(0) * R, len, a.D);
     for (int n = 0; n < n_tiles; ++n) {
-      char* kl = lds + (n & 1) * 2 * Ti::BYTES;
-      char* vl = kl + Ti::BYTES;
-      Ti::put(kl, kreg);
-      Ti::put(vl, vreg);
+      const char* kl = stage.buffer(n);
+      const char* vl = kl + Ti::BYTES;
+      stage.finish(n);
       __syncthreads();
-      if (n + 1 < n_tiles) {
-        Ti::fetch(kreg, kb, a.sk[1], kt.tile(n + 1) * R, len, a.D);
-        Ti::fetch(vreg, vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
-      }
+      if (n + 1 < n_tiles) stage.begin(n + 1, kb, a.sk[1], vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
       const int j0 = kt.tile(n) * R;
       if (w0 >= len) continue;
 #pragma unroll
@@ -411,12 +506,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
           s = Mma<T>::mul(Ti::rows(kl, t * 32, st), qf[st], s);
           p = Mma<T>::mul(Ti::rows(vl, t * 32, st), gf[st], p);
         }
-        const bool whole = all_visible(a, w0, w1, jt, jt + 31, len);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2)) * (p[r] - delta);
-          const int j = jt + acc_row(r);
-          s[r] = whole || (j < len && sees(a, i, j)) ? e : 0.f;
+        for (int r = 0; r < 16; ++r)
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2)) * (p[r] - delta);
+        if (!all_visible(a, w0, w1, jt, jt + 31, len)) {
+          keep_branch();
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = jt + acc_row(r);
+            s[r] = j < len && sees(a, i, j) ? s[r] : 0.f;
+          }
         }
 #pragma unroll
         for (int st = 0; st < Acc<T>::STEPS; ++st) {
@@ -432,150 +531,192 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
 }
 
 // -------------------------------------------------------------------- backward: dk and dv
-// A wave owns 32 keys (columns) and walks over the queries that see them, for every query head of
-// the group in turn, so a shared head's gradient is one sum in registers, in a fixed order.
+// A workgroup owns 128 keys, a wave 32 of them as columns, and walks over the queries that see
+// them, for every query head of the group in turn, so a shared head's gradient is one sum in
+// registers, in a fixed order.
+// dk and dv of a tile are two workgroups, which costs the scores twice (10 D instead of 8 D
+// operations a pair) and is faster: both at once are 2 x 64 accumulators and 2 x 32 registers of
+// keys and values at D = 128, which leaves no room for LDS reads in flight at two waves per SIMD.
 // Key tiles that hold sinks are seen by all later queries: their queries behind the window are
 // given to `nchunks` workgroups more (chunk queries each); all of a split tile's workgroups write
 // fp32 partial results, which attn_join_kernel adds in order.  Without that the one workgroup of
 // the sinks would run T / (left + 128) times as long as any other.
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(const Args a) {
-  constexpr int R = kRows<T>, QT = R / 32;
+struct KeyWork {
+  int tile, part;      // part 0: the window's queries, c + 1: chunk c of those behind it
+  int hk, b, len, k0, lo, hi;
+  bool split, is_dk;
+};
+__device__ __forceinline__ KeyWork key_work(const Args& a) {
+  KeyWork w;
+  // the extra workgroups of the sinks stand evenly between the others
+  const int extra = a.sink_tiles * a.nchunks, items = a.tiles + extra;
+  const TileOf me = tile_of(a, 2 * items, a.right > a.left);
+  const int item = me.tile / 2;
+  w.is_dk = me.tile % 2 == 0;
+  w.hk = me.head % a.Hkv;
+  w.b = me.head / a.Hkv;
+  w.len = length_of(a, w.b);
+  const int before = (int)((int64_t)item * extra / items);   // extra ones before this item
+  if ((int)((int64_t)(item + 1) * extra / items) > before) {
+    w.tile = before / a.nchunks;
+    w.part = before % a.nchunks + 1;
+  } else {
+    w.tile = item - before;
+    w.part = 0;
+  }
+  w.split = w.tile < a.sink_tiles;
+  w.k0 = w.tile * kQueries;
+  const int k1 = min(w.k0 + kQueries, w.len) - 1;
+  w.lo = max(0, w.k0 - a.right);
+  w.hi = min((int64_t)w.len - 1, (int64_t)k1 + a.left);
+  if (w.part > 0) {
+    w.lo = min((int64_t)a.T, (int64_t)w.k0 + kQueries + a.left + (int64_t)(w.part - 1) * a.chunk);
+    w.hi = min((int64_t)w.len - 1, (int64_t)w.lo + a.chunk - 1);
+  } else if (w.split) {
+    w.hi = min((int64_t)w.len - 1, (int64_t)w.k0 + kQueries - 1 + a.left);
+  } else if (w.k0 < a.sinks) {
+    w.hi = w.len - 1;
+  }
+  return w;
+}
+
+// The staged queries of a workgroup: tiles of R rows, head after head.
+template <typename T, int DP, int R, bool DIRECT>
+struct QueryTiles {
+  typedef Stage<T, DP, R, DIRECT, 2 * R * (int)sizeof(float)> St;
+  St stage;
+  int first, per_head, count;
+  float lreg = 0.f, dreg = 0.f;
+  __device__ __forceinline__ void init(const Args& a, const KeyWork& w, char* lds) {
+    first = w.lo / R;
+    per_head = w.hi / R + 1 - first;
+    count = per_head * a.group;
+    stage.init(lds, a.D);
+  }
+  __device__ __forceinline__ int row(int n) const { return (first + n % per_head) * R; }
+  __device__ __forceinline__ void begin(const Args& a, const KeyWork& w, int n) {
+    const int h = w.hk * a.group + n / per_head, r0 = row(n);
+    stage.begin(n, (const T*)a.q + w.b * a.sq[0] + h * a.sq[2], a.sq[1],
+                (const T*)a.grad + ((int64_t)w.b * a.T * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, r0, w.len, a.D);
+    if (threadIdx.x < R) {
+      const int i = r0 + threadIdx.x;
+      const int64_t stat = ((int64_t)w.b * a.Hq + h) * a.T + i;
+      lreg = i < w.len ? a.lse[stat] : INFINITY;   // no query: P = exp2(-inf) = 0
+      dreg = i < w.len ? a.delta[stat] : 0.f;
+    }
+  }
+  __device__ __forceinline__ const char* q(int n) const { return stage.buffer(n); }
+  __device__ __forceinline__ const char* g(int n) const { return stage.buffer(n) + St::Ti::BYTES; }
+  __device__ __forceinline__ float* stats(int n) const {   // lse in log2 units [R], delta [R]
+    return reinterpret_cast<float*>(stage.buffer(n) + 2 * St::Ti::BYTES);
+  }
+  __device__ __forceinline__ void finish(int n) {
+    stage.finish(n);
+    if (threadIdx.x < R) {
+      stats(n)[threadIdx.x] = lreg * kLog2e;
+      stats(n)[R + threadIdx.x] = dreg;
+    }
+  }
+};
+
+template <typename T, int DP, bool DIRECT>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dkv_kernel(const Args a) {
+  constexpr int R = kRows<T>;
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  constexpr int kBuf = 2 * Ti::BYTES + 2 * R * (int)sizeof(float);
-  const uint32_t slot = xcd_slot();
-  const int items = a.tiles + a.sink_tiles * a.nchunks;
-  int item = slot % items;
-  const int hk = slot / items % a.Hkv, b = slot / items / a.Hkv;
-  const int len = length_of(a, b);
-  int tile, part;   // part 0: the window's queries, c + 1: chunk c of those behind it
-  if (item < a.sink_tiles * a.nchunks) {
-    tile = item / a.nchunks;
-    part = item % a.nchunks + 1;
-  } else {
-    tile = item - a.sink_tiles * a.nchunks;
-    part = 0;
-  }
-  const bool split = tile < a.sink_tiles;
+  const KeyWork w = key_work(a);
   const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
-  const int k0 = tile * kQueries, w0 = k0 + wave * 32, j = w0 + lane % 32;
-  const int k1 = min(k0 + kQueries, len) - 1, w1 = min(w0 + 31, len - 1);
-  f32x16 dk[DP / 32], dv[DP / 32];
+  const int w0 = w.k0 + wave * 32, j = w0 + lane % 32, w1 = min(w0 + 31, w.len - 1);
+  f32x16 acc[DP / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = (f32x16)(0.f);
-  // queries of this workgroup
-  int lo = max(0, k0 - a.right), hi = min((int64_t)len - 1, (int64_t)k1 + a.left);
-  if (part > 0) {
-    lo = min((int64_t)a.T, (int64_t)k0 + kQueries + a.left + (int64_t)(part - 1) * a.chunk);
-    hi = min((int64_t)len - 1, (int64_t)lo + a.chunk - 1);
-  } else if (split) {
-    hi = min((int64_t)len - 1, (int64_t)k0 + kQueries - 1 + a.left);
-  } else if (k0 < a.sinks) {
-    hi = len - 1;
-  }
-  if (k0 < len && lo <= hi) {
+  for (int d = 0; d < DP / 32; ++d) acc[d] = (f32x16)(0.f);
+  if (w.k0 < w.len && w.lo <= w.hi) {
     frag kf[Ti::STEPS], vf[Ti::STEPS];
-    own_row<T, DP>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[2] + j * a.sk[1], j < len, a.D);
-    own_row<T, DP>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[2] + j * a.sv[1], j < len, a.D);
-    const int first = lo / R, per_head = hi / R + 1 - first, n_tiles = per_head * a.group;
-    frag qreg[Ti::PER], greg[Ti::PER];
-    float lreg = 0.f, dreg = 0.f;
-    const auto fetch = [&](int n) {
-      const int h = hk * a.group + n / per_head, r0 = (first + n % per_head) * R;
-      Ti::fetch(qreg, (const T*)a.q + b * a.sq[0] + h * a.sq[2], a.sq[1], r0, len, a.D);
-      Ti::fetch(greg, (const T*)a.grad + ((int64_t)b * a.T * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, r0, len,
-                a.D);
-      if (threadIdx.x < R) {
-        const int i = r0 + threadIdx.x;
-        const int64_t stat = ((int64_t)b * a.Hq + h) * a.T + i;
-        lreg = i < len ? a.lse[stat] * kLog2e : INFINITY;
-        dreg = i < len ? a.delta[stat] : 0.f;
-      }
-    };
-    fetch(0);
-    for (int n = 0; n < n_tiles; ++n) {
-      char* ql = lds + (n & 1) * kBuf;
-      char* gl = ql + Ti::BYTES;
-      float* ll = reinterpret_cast<float*>(gl + Ti::BYTES);
-      float* dl = ll + R;
-      Ti::put(ql, qreg);
-      Ti::put(gl, greg);
-      if (threadIdx.x < R) {
-        ll[threadIdx.x] = lreg;
-        dl[threadIdx.x] = dreg;
-      }
+    own_row<T, DP>(kf, (const T*)a.k + w.b * a.sk[0] + w.hk * a.sk[2] + j * a.sk[1], j < w.len, a.D);
+    own_row<T, DP>(vf, (const T*)a.v + w.b * a.sv[0] + w.hk * a.sv[2] + j * a.sv[1], j < w.len, a.D);
+    QueryTiles<T, DP, R, DIRECT> tiles;
+    tiles.init(a, w, lds);
+    tiles.begin(a, w, 0);
+    for (int n = 0; n < tiles.count; ++n) {
+      const char *ql = tiles.q(n), *gl = tiles.g(n);
+      const float* stats = tiles.stats(n);
+      tiles.finish(n);
       __syncthreads();
-      if (n + 1 < n_tiles) fetch(n + 1);
-      const int i0 = (first + n % per_head) * R;
-      if (w0 >= len) continue;
+      if (n + 1 < tiles.count) tiles.begin(a, w, n + 1);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const int it = i0 + t * 32;
+      for (int t = 0; t < R / 32; ++t) {
+        const int it = tiles.row(n) + t * 32;
         // (queries outside [lo, hi] belong to another workgroup of the tile)
-        if (it > hi || it + 31 < lo || none_visible(a, it, it + 31, w0, w1)) continue;
-        f32x16 s = (f32x16)(0.f), p = (f32x16)(0.f);
+        if (w0 >= w.len || it > w.hi || it + 31 < w.lo || none_visible(a, it, it + 31, w0, w1)) continue;
+        f32x16 s = (f32x16)(0.f);
 #pragma unroll
-        for (int st = 0; st < Ti::STEPS; ++st) {
-          s = Mma<T>::mul(Ti::rows(ql, t * 32, st), kf[st], s);
-          p = Mma<T>::mul(Ti::rows(gl, t * 32, st), vf[st], p);
-        }
-        const bool whole = it >= lo && it + 31 <= hi && all_visible(a, it, it + 31, w0, w0 + 31, len);
+        for (int st = 0; st < Ti::STEPS; ++st) s = Mma<T>::mul(Ti::rows(ql, t * 32, st), kf[st], s);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float4_t l2 = *reinterpret_cast<const float4_t*>(ll + t * 32 + g * 8 + lane / 32 * 4);
-          const float4_t de = *reinterpret_cast<const float4_t*>(dl + t * 32 + g * 8 + lane / 32 * 4);
+          const float4_t l2 = *reinterpret_cast<const float4_t*>(stats + t * 32 + g * 8 + lane / 32 * 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e, i = it + acc_row(r);
-            float pe = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2[e]));
-            const float ds = pe * (p[r] - de[e]);
-            const bool see = whole || (i >= lo && i <= hi && j < len && sees(a, i, j));
-            s[r] = see ? pe : 0.f;
-            p[r] = see ? ds : 0.f;
+          for (int e = 0; e < 4; ++e)
+            s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale_log2, -l2[e]));
+        }
+        if (w.is_dk) {
+          f32x16 p = (f32x16)(0.f);
+#pragma unroll
+          for (int st = 0; st < Ti::STEPS; ++st) p = Mma<T>::mul(Ti::rows(gl, t * 32, st), vf[st], p);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4_t de = *reinterpret_cast<const float4_t*>(stats + R + t * 32 + g * 8 + lane / 32 * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] *= p[4 * g + e] - de[e];
           }
         }
+        if (!(it >= w.lo && it + 31 <= w.hi && all_visible(a, it, it + 31, w0, w0 + 31, w.len))) {
+          keep_branch();
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = it + acc_row(r);
+            s[r] = i >= w.lo && i <= w.hi && j < w.len && sees(a, i, j) ? s[r] : 0.f;
+          }
+        }
+        const char* rows = w.is_dk ? ql : gl;
 #pragma unroll
         for (int st = 0; st < Acc<T>::STEPS; ++st) {
-          const frag pf = Acc<T>::operand(s, st), df = Acc<T>::operand(p, st);
+          const frag f = Acc<T>::operand(s, st);
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d) {
-            dv[d] = Mma<T>::mul(Ti::cols(gl, t * 32, st, d * 32), pf, dv[d]);
-            dk[d] = Mma<T>::mul(Ti::cols(ql, t * 32, st, d * 32), df, dk[d]);
-          }
+          for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::mul(Ti::cols(rows, t * 32, st, d * 32), f, acc[d]);
         }
       }
     }
   }
   if (j >= a.T) return;
-  if (split) {
+  const float factor = w.is_dk ? a.scale : 1.f;
+  if (w.split && j < a.sinks) {
     // [b, hk, tile, part, dk / dv, key, D]
-    float* out = a.parts + (((((int64_t)b * a.Hkv + hk) * a.sink_tiles + tile) * (a.nchunks + 1) + part) * 2 *
-                                kQueries + (j - k0)) * a.D;
-    store_columns<float, DP>(out, dk, a.scale, a.D);
-    store_columns<float, DP>(out + (int64_t)kQueries * a.D, dv, 1.f, a.D);
-  } else {
-    const int64_t row = (((int64_t)b * a.T + j) * a.Hkv + hk) * a.D;
-    store_columns<T, DP>((T*)a.dk + row, dk, j < len ? a.scale : 0.f, a.D);
-    store_columns<T, DP>((T*)a.dv + row, dv, j < len ? 1.f : 0.f, a.D);
+    float* out = a.parts + ((((((int64_t)w.b * a.Hkv + w.hk) * a.sink_tiles + w.tile) * (a.nchunks + 1) + w.part) *
+                                 2 + !w.is_dk) * a.sink_rows + (j - w.k0)) * a.D;
+    store_columns<float, DP>(out, acc, factor, a.D);
+  } else if (w.part == 0) {   // (the chunks behind the window concern the sinks alone)
+    T* out = (T*)(w.is_dk ? a.dk : a.dv) + (((int64_t)w.b * a.T + j) * a.Hkv + w.hk) * a.D;
+    store_columns<T, DP>(out, acc, j < w.len ? factor : 0.f, a.D);
   }
 }
 
-// Adds the partial results of the split key tiles in order: one thread per element.
+// Adds the partial results of the sinks in order: one thread per element.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(const Args a, int64_t total) {
   const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (e >= total) return;
-  const int64_t per_tile = (int64_t)kQueries * a.D;
+  const int64_t per_tile = (int64_t)a.sink_rows * a.D;
   const int64_t in_tile = e % per_tile, which = e / per_tile % 2, tile = e / per_tile / 2 % a.sink_tiles;
   const int64_t bh = e / per_tile / 2 / a.sink_tiles;
   const int64_t j = tile * kQueries + in_tile / a.D, b = bh / a.Hkv, hk = bh % a.Hkv;
-  if (j >= a.T) return;
+  if (j >= a.sinks) return;
   const float* p = a.parts + ((bh * a.sink_tiles + tile) * (a.nchunks + 1) * 2 + which) * per_tile + in_tile;
   float s = 0.f;
-  if (j < length_of(a, (int)b))
+  if (j < length_of(a, (int)b)) {
+#pragma unroll 8
     for (int c = 0; c <= a.nchunks; ++c) s += p[(int64_t)c * 2 * per_tile];
+  }
   T* out = (T*)(which ? a.dv : a.dk);
   out[((b * a.T + j) * a.Hkv + hk) * a.D + in_tile % a.D] = (T)s;
 }
@@ -596,9 +737,11 @@ int check(const mn_attention* d) {
 // "No limit" and limits beyond the sequence are T: sums with them stay inside 32 bits.
 int32_t limit(int64_t v, int64_t T) { return (int32_t)(v < 0 || v > T ? T : v); }
 
-// How the queries behind the window of the key tiles with sinks are cut.  A chunk is as long as
-// the window a plain tile walks over, but at most 32 of them; not cut where the sinks are more
-// than an eighth of the keys (enough workgroups share the long walk then).
+// How the queries behind the window of the key tiles with sinks are cut: chunks that make 1024
+// rows to walk over (all heads of the group), longer ones where that would be more than 128
+// chunks.  Shorter ones start and end more often than they multiply (115 chunks of 128 queries at
+// T = 15808, 16 heads of keys: 2.7 ms against 1.9), much longer ones outlast a plain tile.  Not
+// cut where the sinks are more than an eighth of the keys (enough workgroups share the walk then).
 void split_for(const mn_attention* d, Args* a) {
   a->sink_tiles = a->nchunks = 0;
   a->chunk = 1;
@@ -606,16 +749,18 @@ void split_for(const mn_attention* d, Args* a) {
   const int64_t sinks = d->sinks < T ? d->sinks : T, tiles = (sinks + kQueries - 1) / kQueries;
   const int64_t behind = T - kQueries - left;   // queries behind the window of the first tile
   if (sinks == 0 || behind <= 0 || tiles * kQueries * 8 > T) return;
-  int64_t chunk = kQueries + left;
-  if (chunk < (behind + 31) / 32) chunk = (behind + 31) / 32;
+  int64_t chunk = (behind + 127) / 128;
+  const int64_t rows = 1024 / (d->Hq / d->Hkv);
+  chunk = chunk < rows ? rows : chunk;
   chunk = (chunk + 63) / 64 * 64;
   a->sink_tiles = (int32_t)tiles;
+  a->sink_rows = (int32_t)(sinks < kQueries ? sinks : kQueries);
   a->chunk = (int32_t)chunk;
   a->nchunks = (int32_t)((behind + chunk - 1) / chunk);
 }
 
 size_t parts_floats(const mn_attention* d, const Args& a) {
-  return (size_t)d->B * d->Hkv * a.sink_tiles * (a.nchunks + 1) * 2 * kQueries * d->D;
+  return (size_t)d->B * d->Hkv * a.sink_tiles * (a.nchunks + 1) * 2 * a.sink_rows * d->D;
 }
 
 Args args_for(const mn_attention* d) {
@@ -630,22 +775,31 @@ Args args_for(const mn_attention* d) {
   a.sinks = (int32_t)(d->sinks < d->T ? d->sinks : d->T);
   a.tiles = (int32_t)((d->T + kQueries - 1) / kQueries);
   a.group = d->Hq / d->Hkv;
+  a.fold = a.left != a.right && (a.left > a.T / 4 || a.right > a.T / 4);
   a.scale = d->scale;
   a.scale_log2 = d->scale * kLog2e;
   return a;
 }
 
-// f(head size rounded up to 32) as a constant
-template <int V>
+// f(head size rounded up to 32, can rows be loaded straight to LDS) as constants
+template <int V, bool B>
 struct Int {
   static constexpr int value = V;
+  static constexpr bool direct = B;
 };
 template <typename F>
-int for_width(int D, F f) {
-  if (D <= 32) return f(Int<32>());
-  if (D <= 64) return f(Int<64>());
-  if (D <= 96) return f(Int<96>());
-  return f(Int<128>());
+int for_width(int D, bool direct, F f) {
+  if (D <= 32) return direct ? f(Int<32, true>()) : f(Int<32, false>());
+  if (D <= 64) return direct ? f(Int<64, true>()) : f(Int<64, false>());
+  if (D <= 96) return direct ? f(Int<96, true>()) : f(Int<96, false>());
+  return direct ? f(Int<128, true>()) : f(Int<128, false>());
+}
+
+// Loads straight to LDS move 16-byte chunks: rows have to start on 16 bytes and be whole chunks.
+bool direct_rows(const void* p, const int64_t* stride, const mn_attention* d, int bytes) {
+  const int64_t n = 16 / bytes;
+  return mn_aligned(p, 16) && d->D % n == 0 && (d->B == 1 || stride[0] % n == 0) &&
+         (d->T == 1 || stride[1] % n == 0) && stride[2] % n == 0;
 }
 
 // Dynamic LDS of more than 64 KB has to be asked for, once per kernel and device.
@@ -660,14 +814,16 @@ constexpr int kLdsQ = 4 * Tile<T, DP, kRows<T>>::BYTES;   // two buffers of two 
 template <typename T, int DP>
 constexpr int kLdsKv = kLdsQ<T, DP> + 4 * kRows<T> * (int)sizeof(float);   // and two rows' statistics
 
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 bool init_one() {
-  return raise_lds(attn_fwd_kernel<T, DP>, kLdsQ<T, DP>) && raise_lds(attn_dq_kernel<T, DP>, kLdsQ<T, DP>) &&
-         raise_lds(attn_dkv_kernel<T, DP>, kLdsKv<T, DP>);
+  return raise_lds(attn_fwd_kernel<T, DP, DIRECT>, kLdsQ<T, DP>) && raise_lds(attn_dq_kernel<T, DP, DIRECT>, kLdsQ<T, DP>) &&
+         raise_lds(attn_dkv_kernel<T, DP, DIRECT>, kLdsKv<T, DP>);
 }
 template <typename T>
 bool init_type() {
-  return init_one<T, 32>() && init_one<T, 64>() && init_one<T, 96>() && init_one<T, 128>();
+  return init_one<T, 32, false>() && init_one<T, 64, false>() && init_one<T, 96, false>() &&
+         init_one<T, 128, false>() && init_one<T, 32, true>() && init_one<T, 64, true>() &&
+         init_one<T, 96, true>() && init_one<T, 128, true>();
 }
 
 }  // namespace
@@ -689,10 +845,12 @@ int mn_attention_fwd(const mn_attention* d, const void* q, const void* k, const 
     Args a = args_for(d);
     a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse; a.lengths = lengths;
     const unsigned grid = (unsigned)(a.tiles * d->Hq * d->B);
-    return for_width(d->D, [&](auto w) {
+    const bool direct = direct_rows(k, a.sk, d, sizeof(T)) && direct_rows(v, a.sv, d, sizeof(T));
+    return for_width(d->D, direct, [&](auto w) {
       constexpr int DP = decltype(w)::value, lds = kLdsQ<T, DP>;
-      if (!raise_lds(attn_fwd_kernel<T, DP>, lds)) return (int)MN_ELAUNCH;
-      attn_fwd_kernel<T, DP><<<grid, kThreads, lds, mn_stream(stream)>>>(a);
+      constexpr bool DIRECT = decltype(w)::direct;
+      if (!raise_lds(attn_fwd_kernel<T, DP, DIRECT>, lds)) return (int)MN_ELAUNCH;
+      attn_fwd_kernel<T, DP, DIRECT><<<grid, kThreads, lds, mn_stream(stream)>>>(a);
       return mn_launch_status();
     });
   });
@@ -722,17 +880,20 @@ int mn_attention_bwd(const mn_attention* d, const void* grad, const void* q, con
     a.parts = a.delta + (size_t)d->B * d->Hq * d->T;
     split_for(d, &a);
     hipStream_t s = mn_stream(stream);
-    const int rc = for_width(d->D, [&](auto w) {
+    const bool direct = direct_rows(k, a.sk, d, sizeof(T)) && direct_rows(v, a.sv, d, sizeof(T)) &&
+                        direct_rows(q, a.sq, d, sizeof(T)) && mn_aligned(grad, 16);
+    const int rc = for_width(d->D, direct, [&](auto w) {
+      constexpr bool DIRECT = decltype(w)::direct;
       constexpr int DP = decltype(w)::value, lds_q = kLdsQ<T, DP>, lds_kv = kLdsKv<T, DP>;
-      if (!raise_lds(attn_dq_kernel<T, DP>, lds_q) || !raise_lds(attn_dkv_kernel<T, DP>, lds_kv))
+      if (!raise_lds(attn_dq_kernel<T, DP, DIRECT>, lds_q) || !raise_lds(attn_dkv_kernel<T, DP, DIRECT>, lds_kv))
         return (int)MN_ELAUNCH;
-      attn_dq_kernel<T, DP><<<(unsigned)(a.tiles * d->Hq * d->B), kThreads, lds_q, s>>>(a);
+      attn_dq_kernel<T, DP, DIRECT><<<(unsigned)(a.tiles * d->Hq * d->B), kThreads, lds_q, s>>>(a);
       const unsigned items = (unsigned)(a.tiles + a.sink_tiles * a.nchunks);
-      attn_dkv_kernel<T, DP><<<(unsigned)(items * d->Hkv * d->B), kThreads, lds_kv, s>>>(a);
+      attn_dkv_kernel<T, DP, DIRECT><<<(unsigned)(2 * items * d->Hkv * d->B), kThreads, lds_kv, s>>>(a);
       return mn_launch_status();
     });
     if (rc != MN_OK || !a.sink_tiles) return rc;
-    const int64_t total = d->B * d->Hkv * a.sink_tiles * 2 * kQueries * d->D;
+    const int64_t total = d->B * d->Hkv * a.sink_tiles * 2 * a.sink_rows * d->D;
     attn_join_kernel<T><<<(unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, total);
     return mn_launch_status();
   });

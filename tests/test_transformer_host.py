@@ -136,12 +136,12 @@ def test_attention_workspace():
     rows = 4 * 2 * 4          # fp32 per token: batch 2, 4 heads
     assert size() == rows * 300 and size(sinks=0) == rows * 300 and size(left=-1, T=5000) == rows * 5000
     assert size(T=0) == 0 and size(D=129) == 0
-    # sinks behind a window: partial results of at most 33 workgroups per tile of 128 keys
+    # sinks behind a window: partial results of at most 129 workgroups per sink
     for T, left, sinks in ((1100, 60, 1), (15808, 1024, 4), (1 << 20, 0, 200), (40000, 128, 4000)):
         parts = size(T=T, left=left, sinks=sinks) - rows * T
-        tile = 2 * 2 * 2 * 128 * 64 * 4   # batch, key heads, dk and dv
-        tiles = (sinks + 127) // 128
-        assert parts % (tile * tiles) == 0 and 2 <= parts // (tile * tiles) <= 33, (T, left, sinks)
+        key = 2 * 2 * 2 * 64 * 4          # batch, key heads, dk and dv
+        kept = sinks if sinks < 128 else (sinks + 127) // 128 * 128
+        assert parts % (key * kept) == 0 and 2 <= parts // (key * kept) <= 129, (T, left, sinks)
     assert size(T=2000, left=10, sinks=300) == rows * 2000   # more than an eighth of the keys
 
 
