@@ -77,25 +77,35 @@ struct Mma<float> {   // four contraction slots a lane: four instructions of two
   }
 };
 
-// 16 bytes a lane from memory to LDS (wave-uniform address `lds` + 16 * lane), asynchronous: the
-// data is there after wait_loads() and a barrier.  In assembly because the compiler, which cannot
-// tell the two buffers apart, would wait for the load before the next read of LDS; m0 is put back.
-__device__ __forceinline__ void load_to_lds(const void* p, uint32_t lds) {
+// 16 bytes a lane from memory (uniform address + 32-bit offset) to LDS (wave-uniform address +
+// 16 * lane), asynchronous: the data is there after wait_loads() and a barrier.  In assembly
+// because the compiler, which cannot tell the two buffers apart, would wait for the load before
+// the next read of LDS; m0 is put back.
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, uint32_t lds) {
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
                "s_mov_b32 m0, %0"
                : "=&s"(m0)
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base)
                : "memory");
 }
-// Keeps the scheduler from sinking loads to their uses: several LDS reads are in flight while
-// earlier ones are multiplied.
-__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const char* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
-
+// The order of a block of N products, each fed by READS reads of LDS: reads run AHEAD products
+// before their use.  (Left alone, the compiler reads right before each product and waits.)
+template <int N, int READS, int AHEAD>
+__device__ __forceinline__ void feed() {
+  constexpr int kMfma = 0x8, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kRead, READS * AHEAD, 0);
+#pragma unroll
+  for (int k = 0; k < N - AHEAD; ++k) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, AHEAD, 0);
+}
 // One tile of rows in LDS: DP elements a row (D rounded up to 32, zeros behind D).
 template <typename T, int DP, int ROWS>
 struct Tile {
@@ -149,13 +159,21 @@ struct Tile {
   // instruction in the order of the lanes, so the swizzle is in which chunk a lane asks for.
   // Rows from `end` on repeat the last one: what is multiplied with them is zero.  Needs
   // 16-byte aligned rows of whole chunks; chunks behind D are not written (see clear).
-  static __device__ __forceinline__ void load(uint32_t lds, const T* base, int64_t stride, int r0, int end,
-                                              int D) {
+  static constexpr int SLOTS = ROWS * NC / kThreads;
+  static __device__ __forceinline__ uint32_t offset(int p, int rows, int64_t stride) {
+    const int slot = threadIdx.x + p * kThreads, row = min(slot / NC, rows - 1), chunk = slot % NC ^ swz(slot / NC);
+    return (uint32_t)((row * stride + chunk * N) * (int)sizeof(T));
+  }
+  // `offsets`: those of a whole tile, which a thread keeps
+  static __device__ __forceinline__ void load(uint32_t lds, const T* rows, const uint32_t* offsets, int64_t stride,
+                                              int left, int D) {
 #pragma unroll
-    for (int p = 0; p < ROWS * NC / kThreads; ++p) {
-      const int slot = threadIdx.x + p * kThreads, row = slot / NC, chunk = slot % NC ^ swz(row);
+    for (int p = 0; p < SLOTS; ++p) {
+      const int slot = threadIdx.x + p * kThreads, chunk = slot % NC ^ swz(slot / NC);
       const uint32_t at = lds + (p * kThreads + (threadIdx.x & ~(MN_WAVE - 1))) * 16;
-      if (chunk * N < D) load_to_lds(base + min(r0 + row, end - 1) * stride + chunk * N, at);
+      uint32_t off = offsets[p];
+      if (left < ROWS) off = offset(p, left, stride);
+      if (D == NC * N || chunk * N < D) load_to_lds((const char*)rows, off, at);
     }
   }
   static __device__ __forceinline__ void clear(char* lds, int D) {
@@ -207,23 +225,30 @@ struct Stage {
   static constexpr int kBuf = 2 * Ti::BYTES + EXTRA;
   char* lds;
   typename Ti::frag r0[DIRECT ? 1 : Ti::PER], r1[DIRECT ? 1 : Ti::PER];
+  uint32_t o0[DIRECT ? Ti::SLOTS : 1], o1[DIRECT ? Ti::SLOTS : 1];
 
   __device__ __forceinline__ char* buffer(int n) const { return lds + (n & 1) * kBuf; }
-  __device__ __forceinline__ void init(char* p, int D) {
+  __device__ __forceinline__ void init(char* p, int64_t sa, int64_t sb, int D) {
     lds = p;
-    if (DIRECT)
+    if constexpr (DIRECT) {
+#pragma unroll
+      for (int k = 0; k < Ti::SLOTS; ++k) {
+        o0[k] = Ti::offset(k, ROWS, sa);
+        o1[k] = Ti::offset(k, ROWS, sb);
+      }
       for (int n = 0; n < 2; ++n) {
         Ti::clear(buffer(n), D);
         Ti::clear(buffer(n) + Ti::BYTES, D);
       }
+    }
   }
   // tile n: rows row0 .. of two heads
   __device__ __forceinline__ void begin(int n, const T* a, int64_t sa, const T* b, int64_t sb, int row0,
                                         int end, int D) {
     if constexpr (DIRECT) {
       const uint32_t at = lds_address(buffer(n));
-      Ti::load(at, a, sa, row0, end, D);
-      Ti::load(at + Ti::BYTES, b, sb, row0, end, D);
+      Ti::load(at, a + row0 * sa, o0, sa, end - row0, D);
+      Ti::load(at + Ti::BYTES, b + row0 * sb, o1, sb, end - row0, D);
     } else {
       Ti::fetch(r0, a, sa, row0, end, D);
       Ti::fetch(r1, b, sb, row0, end, D);
@@ -384,7 +409,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
     const KeyTiles kt = key_tiles<R>(a, q0, min(q0 + kQueries, len) - 1, len);
     const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
     Stage<T, DP, R, DIRECT, 0> stage;
-    stage.init(lds, a.D);
+    stage.init(lds, a.sk[1], a.sv[1], a.D);
     stage.begin(0, kb, a.sk[1], vb, a.sv[1], kt.tile(0) * R, len, a.D);
     for (int n = 0; n < n_tiles; ++n) {
       const char* kl = stage.buffer(n);
@@ -402,6 +427,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
         s[t] = (f32x16)(0.f);
 #pragma unroll
         for (int st = 0; st < Ti::STEPS; ++st) s[t] = Mma<T>::mul(Ti::rows(kl, t * 32, st), qf[st], s[t]);
+        if constexpr (sizeof(T) == 2) feed<Ti::STEPS, 1, 4 < Ti::STEPS ? 4 : Ti::STEPS>();
         if (!whole) {
           keep_branch();
 #pragma unroll
@@ -486,7 +512,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
     const KeyTiles kt = key_tiles<R>(a, q0, min(q0 + kQueries, len) - 1, len);
     const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
     Stage<T, DP, R, DIRECT, 0> stage;
-    stage.init(lds, a.D);
+    stage.init(lds, a.sk[1], a.sv[1], a.D);
     stage.begin(0, kb, a.sk[1], vb, a.sv[1], kt.tile(0) * R, len, a.D);
     for (int n = 0; n < n_tiles; ++n) {
       const char* kl = stage.buffer(n);
@@ -506,6 +532,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
           s = Mma<T>::mul(Ti::rows(kl, t * 32, st), qf[st], s);
           p = Mma<T>::mul(Ti::rows(vl, t * 32, st), gf[st], p);
         }
+        if constexpr (sizeof(T) == 2) feed<2 * Ti::STEPS, 1, 4>();
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2)) * (p[r] - delta);
@@ -524,6 +551,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
           for (int d = 0; d < DP / 32; ++d)
             acc[d] = Mma<T>::mul(Ti::cols(kl, t * 32, st, d * 32), ds, acc[d]);
         }
+        if constexpr (sizeof(T) == 2) feed<Acc<T>::STEPS * DP / 32, 2, 2>();
       }
     }
   }
@@ -585,24 +613,29 @@ template <typename T, int DP, int R, bool DIRECT>
 struct QueryTiles {
   typedef Stage<T, DP, R, DIRECT, 2 * R * (int)sizeof(float)> St;
   St stage;
-  int first, per_head, count;
+  int count, row;                   // tiles; first row of the one that was finished last
+  int first, head, next, pending;   // what begin() will load, what it has begun
   float lreg = 0.f, dreg = 0.f;
   __device__ __forceinline__ void init(const Args& a, const KeyWork& w, char* lds) {
-    first = w.lo / R;
-    per_head = w.hi / R + 1 - first;
-    count = per_head * a.group;
-    stage.init(lds, a.D);
+    first = next = w.lo / R * R;
+    count = (w.hi / R + 1 - w.lo / R) * a.group;
+    head = w.hk * a.group;
+    stage.init(lds, a.sq[1], (int64_t)a.Hq * a.D, a.D);
   }
-  __device__ __forceinline__ int row(int n) const { return (first + n % per_head) * R; }
   __device__ __forceinline__ void begin(const Args& a, const KeyWork& w, int n) {
-    const int h = w.hk * a.group + n / per_head, r0 = row(n);
-    stage.begin(n, (const T*)a.q + w.b * a.sq[0] + h * a.sq[2], a.sq[1],
-                (const T*)a.grad + ((int64_t)w.b * a.T * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, r0, w.len, a.D);
+    pending = next;
+    stage.begin(n, (const T*)a.q + w.b * a.sq[0] + head * a.sq[2], a.sq[1],
+                (const T*)a.grad + ((int64_t)w.b * a.T * a.Hq + head) * a.D, (int64_t)a.Hq * a.D, next, w.len, a.D);
     if (threadIdx.x < R) {
-      const int i = r0 + threadIdx.x;
-      const int64_t stat = ((int64_t)w.b * a.Hq + h) * a.T + i;
+      const int i = next + threadIdx.x;
+      const int64_t stat = ((int64_t)w.b * a.Hq + head) * a.T + i;
       lreg = i < w.len ? a.lse[stat] : INFINITY;   // no query: P = exp2(-inf) = 0
       dreg = i < w.len ? a.delta[stat] : 0.f;
+    }
+    next += R;
+    if (next > w.hi) {
+      next = first;
+      ++head;
     }
   }
   __device__ __forceinline__ const char* q(int n) const { return stage.buffer(n); }
@@ -612,6 +645,7 @@ struct QueryTiles {
   }
   __device__ __forceinline__ void finish(int n) {
     stage.finish(n);
+    row = pending;
     if (threadIdx.x < R) {
       stats(n)[threadIdx.x] = lreg * kLog2e;
       stats(n)[R + threadIdx.x] = dreg;
@@ -643,15 +677,17 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
       const float* stats = tiles.stats(n);
       tiles.finish(n);
       __syncthreads();
+      const int row0 = tiles.row;
       if (n + 1 < tiles.count) tiles.begin(a, w, n + 1);
 #pragma unroll
       for (int t = 0; t < R / 32; ++t) {
-        const int it = tiles.row(n) + t * 32;
+        const int it = row0 + t * 32;
         // (queries outside [lo, hi] belong to another workgroup of the tile)
         if (w0 >= w.len || it > w.hi || it + 31 < w.lo || none_visible(a, it, it + 31, w0, w1)) continue;
         f32x16 s = (f32x16)(0.f);
 #pragma unroll
         for (int st = 0; st < Ti::STEPS; ++st) s = Mma<T>::mul(Ti::rows(ql, t * 32, st), kf[st], s);
+        if constexpr (sizeof(T) == 2) feed<Ti::STEPS, 1, 4 < Ti::STEPS ? 4 : Ti::STEPS>();
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4_t l2 = *reinterpret_cast<const float4_t*>(stats + t * 32 + g * 8 + lane / 32 * 4);
@@ -663,6 +699,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
           f32x16 p = (f32x16)(0.f);
 #pragma unroll
           for (int st = 0; st < Ti::STEPS; ++st) p = Mma<T>::mul(Ti::rows(gl, t * 32, st), vf[st], p);
+          if constexpr (sizeof(T) == 2) feed<Ti::STEPS, 1, 4 < Ti::STEPS ? 4 : Ti::STEPS>();
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float4_t de = *reinterpret_cast<const float4_t*>(stats + R + t * 32 + g * 8 + lane / 32 * 4);
@@ -685,6 +722,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::mul(Ti::cols(rows, t * 32, st, d * 32), f, acc[d]);
         }
+        if constexpr (sizeof(T) == 2) feed<Acc<T>::STEPS * DP / 32, 2, 2>();
       }
     }
   }
@@ -798,8 +836,8 @@ int for_width(int D, bool direct, F f) {
 // Loads straight to LDS move 16-byte chunks: rows have to start on 16 bytes and be whole chunks.
 bool direct_rows(const void* p, const int64_t* stride, const mn_attention* d, int bytes) {
   const int64_t n = 16 / bytes;
-  return mn_aligned(p, 16) && d->D % n == 0 && (d->B == 1 || stride[0] % n == 0) &&
-         (d->T == 1 || stride[1] % n == 0) && stride[2] % n == 0;
+  return mn_aligned(p, 16) && d->D % n == 0 && (d->B == 1 || stride[0] % n == 0) && stride[1] % n == 0 &&
+         stride[2] % n == 0 && stride[1] >= 0 && stride[1] < (1 << 22);   // 64 rows in 31 bits
 }
 
 // Dynamic LDS of more than 64 KB has to be asked for, once per kernel and device.
@@ -881,7 +919,8 @@ int mn_attention_bwd(const mn_attention* d, const void* grad, const void* q, con
     split_for(d, &a);
     hipStream_t s = mn_stream(stream);
     const bool direct = direct_rows(k, a.sk, d, sizeof(T)) && direct_rows(v, a.sv, d, sizeof(T)) &&
-                        direct_rows(q, a.sq, d, sizeof(T)) && mn_aligned(grad, 16);
+                        direct_rows(q, a.sq, d, sizeof(T)) && mn_aligned(grad, 16) &&
+                        (int64_t)d->Hq * d->D < (1 << 22);
     const int rc = for_width(d->D, direct, [&](auto w) {
       constexpr bool DIRECT = decltype(w)::direct;
       constexpr int DP = decltype(w)::value, lds_q = kLdsQ<T, DP>, lds_kv = kLdsKv<T, DP>;
