@@ -279,18 +279,31 @@ struct Acc {
   }
 };
 
-// Row of an accumulator's register r.
-__device__ __forceinline__ int acc_row(int r) {
-  return r / 4 * 8 + (int)(threadIdx.x % MN_WAVE / 32) * 4 + r % 4;
-}
+// Row of an accumulator's register r, less the 4 of a lane of the upper half.
+__device__ __forceinline__ constexpr int acc_row(int r) { return r / 4 * 8 + r % 4; }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, MN_WAVE); }
 
 // In a branch few tiles take: keeps the compiler from computing both sides for all of them.
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
-__device__ __forceinline__ bool sees(const Args& a, int i, int j) {
-  return j <= i + a.right && (j >= i - a.left || j < a.sinks);
+// What a lane's query sees of a tile, or which of a tile's queries see a lane's key, for the row
+// numbers of an accumulator (constants c = r / 4 * 8 + r % 4; the lane's half is in the bounds):
+// one interval, and the first few.
+struct Seen {
+  int lo, first;
+  unsigned span;
+  __device__ __forceinline__ bool operator()(int c) const { return (unsigned)(c - lo) <= span || c < first; }
+};
+__device__ __forceinline__ Seen interval(int lo, int hi, int first, int row0) {
+  const int base = row0 + (int)(threadIdx.x % MN_WAVE / 32) * 4;
+  if (hi < lo) return {1 << 30, first - base, 0u};
+  return {lo - base, first - base, (unsigned)(hi - lo)};
+}
+// keys of query i in the tile that starts at j0 (sinks end where the others do)
+__device__ __forceinline__ Seen keys_seen(const Args& a, int i, int j0, int len) {
+  const int hi = min(i + a.right, len - 1);
+  return interval(max(i - a.left, 0), hi, min(a.sinks, hi + 1), j0);
 }
 
 // Where the keys of queries q0 .. q1 lie: tiles [0, sinks) and [first, last) of ROWS keys.
@@ -430,11 +443,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
         if constexpr (sizeof(T) == 2) feed<Ti::STEPS, 1, 4 < Ti::STEPS ? 4 : Ti::STEPS>();
         if (!whole) {
           keep_branch();
+          const Seen see = keys_seen(a, i, j0 + t * 32, len);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = j0 + t * 32 + acc_row(r);
-            s[t][r] = j < len && sees(a, i, j) ? s[t][r] : -INFINITY;
-          }
+          for (int r = 0; r < 16; ++r) s[t][r] = see(acc_row(r)) ? s[t][r] : -INFINITY;
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
@@ -538,11 +549,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
           s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -l2)) * (p[r] - delta);
         if (!all_visible(a, w0, w1, jt, jt + 31, len)) {
           keep_branch();
+          const Seen see = keys_seen(a, i, jt, len);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = jt + acc_row(r);
-            s[r] = j < len && sees(a, i, j) ? s[r] : 0.f;
-          }
+          for (int r = 0; r < 16; ++r) s[r] = see(acc_row(r)) ? s[r] : 0.f;
         }
 #pragma unroll
         for (int st = 0; st < Acc<T>::STEPS; ++st) {
@@ -709,11 +718,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
         }
         if (!(it >= w.lo && it + 31 <= w.hi && all_visible(a, it, it + 31, w0, w0 + 31, w.len))) {
           keep_branch();
+          const int last = j < a.sinks ? w.hi : min(w.hi, j + a.left);
+          const Seen see = interval(max(w.lo, j - a.right), j < w.len ? last : -1, 0, it);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = it + acc_row(r);
-            s[r] = i >= w.lo && i <= w.hi && j < w.len && sees(a, i, j) ? s[r] : 0.f;
-          }
+          for (int r = 0; r < 16; ++r) s[r] = see(acc_row(r)) ? s[r] : 0.f;
         }
         const char* rows = w.is_dk ? ql : gl;
 #pragma unroll
