@@ -12,7 +12,7 @@
 // Orientation.  A 32x32 accumulator holds one COLUMN per lane (lane l: column l % 32, of its 32
 // rows the 16 with bit 2 equal to l / 32).  Scores are computed transposed where a row of the
 // softmax runs over keys (S^T = K Q^T: a lane owns one query, so maximum and sum are a fold over
-// registers and one exchange with lane l ^ 32), and the accumulator's registers are, in order,
+// registers and one swap with lane l ^ 32), and the accumulator's registers are, in order,
 // the B operand of the next product over the same 32 keys (or queries): which of the 32 a slot of
 // the contraction means is free as long as A uses the same assignment, and the A operand is read
 // from LDS for exactly those.  P and dS therefore never leave the registers of their lane.
@@ -282,8 +282,6 @@ struct Acc {
 // Row of an accumulator's register r, less the 4 of a lane of the upper half.
 __device__ __forceinline__ constexpr int acc_row(int r) { return r / 4 * 8 + r % 4; }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, MN_WAVE); }
-
 // In a branch few tiles take: keeps the compiler from computing both sides for all of them.
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
@@ -450,7 +448,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
       }
-      top = fmaxf(top, other_half(top)) * a.scale_log2;
+      top = max_xor32(top) * a.scale_log2;
       // a new maximum only where the old one is left behind by more than 2^8: below that P stays
       // below 2^8 and nothing has to be scaled
       if (__any(top > m + 8.f)) {
@@ -481,7 +479,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
     }
   }
   if (i >= a.T) return;
-  sum += other_half(sum);
+  sum = plus_xor32(sum);
   const bool any = i < len && m != -INFINITY;   // (a NaN among the scores: m may be -inf, sum is NaN)
   const bool valid = i < len && (any || sum != sum);
   store_columns<T, DP>(orow, acc, valid ? 1.f / sum : 0.f, a.D);
@@ -514,7 +512,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
     for (int s = 0; s < Ti::STEPS; ++s)
 #pragma unroll
       for (int e = 0; e < Ti::N; ++e) delta += (float)qf[s][e] * (float)gf[s][e];
-    delta += other_half(delta);
+    delta = plus_xor32(delta);
     if (i < len && lane < 32) a.delta[stat] = delta;
     const float l2 = i < len ? a.lse[stat] * kLog2e : INFINITY;   // no query: P = exp2(-inf) = 0
     own_row<T, DP>(qf, (const T*)a.q + b * a.sq[0] + h * a.sq[2] + i * a.sq[1], i < len, a.D);

@@ -16,6 +16,16 @@ struct Vec16 {
   typedef T utype __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
+// `cnt` (0..N) elements from p, zeros behind them.
+template <typename T>
+__device__ __forceinline__ typename Vec16<T>::type load_raw(const T* p, int cnt) {
+  if (cnt == Vec16<T>::N) return *reinterpret_cast<const typename Vec16<T>::utype*>(p);
+  typename Vec16<T>::type v;
+#pragma unroll
+  for (int e = 0; e < Vec16<T>::N; ++e) v[e] = e < cnt ? p[e] : (T)0.f;
+  return v;
+}
+
 // `cnt` (0..N) elements from p as fp32, zeros behind them.
 template <typename T>
 __device__ __forceinline__ void load_vec(const T* p, int cnt, float* out) {
@@ -44,6 +54,37 @@ __device__ __forceinline__ void store_vec(T* p, int cnt, const float* in) {
     for (int e = 0; e < N; ++e)
       if (e < cnt) p[e] = (T)in[e];
   }
+}
+
+// v of lane l plus v of lane l ^ 32 (or l ^ 16), without LDS.
+__device__ __forceinline__ float plus_xor32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float plus_xor16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_xor32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int CTRL>
+__device__ __forceinline__ float plus_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// Sum over groups of LANES (8 .. 64) neighbouring lanes, in every lane of the group: within 16
+// lanes by DPP (neighbour, pair, mirrored half row, mirrored row), across them by lane swaps - a
+// few cycles each where a shuffle through LDS takes a hundred.  A group reads its own lanes only.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+  v = plus_dpp<0xB1>(v);
+  v = plus_dpp<0x4E>(v);
+  v = plus_dpp<0x141>(v);
+  if (LANES > 8) v = plus_dpp<0x140>(v);
+  if (LANES > 16) v = plus_xor16(v);
+  if (LANES > 32) v = plus_xor32(v);
+  return v;
 }
 
 // Calls f with a value of the element type that `dtype` names; MN_EUNSUPPORTED for others.

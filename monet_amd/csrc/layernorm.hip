@@ -8,7 +8,8 @@
 // so a row far off zero loses nothing.  LANES lanes share a row: part of a wave for short rows
 // (several rows a wave), a wave up to 2048 elements, a workgroup above; the groups walk over the
 // rows with w and b in registers, so those are read once per group and not once per row (with
-// fp32 weights next to 16-bit rows they are twice the bytes of the row).
+// fp32 weights next to 16-bit rows they are twice the bytes of the row), and load the next row
+// before they work on one.
 // Backward sums dw and db over a group's rows in registers, over a workgroup's groups in a fixed
 // order, and writes one partial row per workgroup; a second kernel adds those in a fixed order:
 // no atomics, the same bits every run.  All sums are fp32.
@@ -16,14 +17,13 @@
 
 namespace {
 
-constexpr int kMaxParts = 1024;   // partial rows of dw / db at most
+constexpr int kMaxParts = 1024;    // partial rows of dw / db at most
+constexpr int kMaxBlocks = 1024;   // forward: four workgroups a CU
 
 // Sum over the LANES lanes (or threads) of a group; every lane gets the total.
 template <int LANES>
 __device__ __forceinline__ float group_sum(float v, float* lds) {
-  constexpr int W = LANES < MN_WAVE ? LANES : MN_WAVE;
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, MN_WAVE);
+  v = lane_sum<(LANES < MN_WAVE ? LANES : MN_WAVE)>(v);
   if (LANES > MN_WAVE) {
     __syncthreads();   // the previous sum has been read
     if (threadIdx.x % MN_WAVE == 0) lds[threadIdx.x / MN_WAVE] = v;
@@ -38,12 +38,8 @@ __device__ __forceinline__ float group_sum(float v, float* lds) {
 // Two sums at once: one wait for both.
 template <int LANES>
 __device__ __forceinline__ void group_sum2(float& a, float& b, float* lds) {
-  constexpr int W = LANES < MN_WAVE ? LANES : MN_WAVE;
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) {
-    a += __shfl_xor(a, o, MN_WAVE);
-    b += __shfl_xor(b, o, MN_WAVE);
-  }
+  a = lane_sum<(LANES < MN_WAVE ? LANES : MN_WAVE)>(a);
+  b = lane_sum<(LANES < MN_WAVE ? LANES : MN_WAVE)>(b);
   if (LANES > MN_WAVE) {
     __syncthreads();
     if (threadIdx.x % MN_WAVE == 0) {
@@ -71,6 +67,21 @@ __device__ __forceinline__ int chunk_cnt(int64_t D, int col) {
   return left >= N ? N : (left > 0 ? (int)left : 0);
 }
 
+// A lane's part of a row, as it lies in memory.
+template <typename T, int LANES, int NE>
+struct RowPart {
+  static constexpr int N = Vec16<T>::N;
+  typename Vec16<T>::type v[NE / N];
+  __device__ __forceinline__ void load(const T* row, int64_t D, int lane) {
+#pragma unroll
+    for (int c = 0; c < NE / N; ++c) {
+      const int col = chunk_col<LANES, N>(lane, c);
+      v[c] = load_raw<T>(row + col, chunk_cnt<N>(D, col));   // zeros behind the row
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const { return (float)v[e / N][e % N]; }
+};
+
 // NE weights of a lane as fp32 (`none` where there is no weight tensor).
 template <typename W, int LANES, int NE, int N>
 __device__ __forceinline__ void load_weights(const W* w, int64_t D, int lane, float none, float* out) {
@@ -84,28 +95,30 @@ __device__ __forceinline__ void load_weights(const W* w, int64_t D, int lane, fl
 }
 
 template <typename T, typename W, int LANES, int NE>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(
+__global__ __launch_bounds__(LANES > 64 ? LANES : 256) void ln_fwd_kernel(
     const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y,
     float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int64_t D, float dim,
     float eps) {
-  constexpr int N = Vec16<T>::N, TPB = LANES > 256 ? LANES : 256, G = TPB / LANES;
+  constexpr int N = Vec16<T>::N, TPB = LANES > 64 ? LANES : 256, G = TPB / LANES;
   __shared__ float lds[2 * TPB / MN_WAVE];
   const int lane = threadIdx.x % LANES;
   float wr[NE], br[NE];
   load_weights<W, LANES, NE, N>(w, D, lane, 1.f, wr);
   load_weights<W, LANES, NE, N>(b, D, lane, 0.f, br);
-  for (int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / LANES; row < rows;
-       row += (int64_t)gridDim.x * G) {
-    const T* xr = x + row * D;
+  // (the next row is on its way while this one is worked on)
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / LANES;
+  RowPart<T, LANES, NE> ahead;
+  if (row < rows) ahead.load(x + row * D, D, lane);
+  for (; row < rows; row += step) {
     float v[NE];
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < NE / N; ++c) {
-      const int col = chunk_col<LANES, N>(lane, c);
-      load_vec<T>(xr + col, chunk_cnt<N>(D, col), v + c * N);
+    for (int e = 0; e < NE; ++e) {
+      v[e] = ahead[e];
+      s += v[e];
     }
-#pragma unroll
-    for (int e = 0; e < NE; ++e) s += v[e];
+    if (row + step < rows) ahead.load(x + (row + step) * D, D, lane);
     const float mu = group_sum<LANES>(s, lds) / dim;
     s = 0.f;
 #pragma unroll
@@ -136,29 +149,41 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_fwd_kernel(
 
 // parts == nullptr: the only workgroup, which writes dw / db itself.
 template <typename T, typename W, int LANES, int NE>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(
+__global__ __launch_bounds__(LANES > 64 ? LANES : 256) void ln_bwd_kernel(
     const T* __restrict__ g, const T* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const W* __restrict__ w, T* __restrict__ dx,
     float* __restrict__ parts, W* __restrict__ dw, W* __restrict__ db, int64_t rows, int64_t D,
     float dim) {
-  constexpr int N = Vec16<T>::N, TPB = LANES > 256 ? LANES : 256, G = TPB / LANES;
+  constexpr int N = Vec16<T>::N, TPB = LANES > 64 ? LANES : 256, G = TPB / LANES;
   __shared__ float lds[2 * TPB / MN_WAVE];
   const int lane = threadIdx.x % LANES;
   float wr[NE], aw[NE], ab[NE];
   load_weights<W, LANES, NE, N>(w, D, lane, 1.f, wr);
 #pragma unroll
   for (int e = 0; e < NE; ++e) aw[e] = ab[e] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / LANES; row < rows;
-       row += (int64_t)gridDim.x * G) {
-    const T* xr = x + row * D;
-    const T* gr = g + row * D;
-    const float mu = mean[row], r = rstd[row];
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / LANES;
+  RowPart<T, LANES, NE> xa, ga;   // the next row; zeros behind it add nothing below
+  float mu_a = 0.f, r_a = 0.f;
+  if (row < rows) {
+    xa.load(x + row * D, D, lane);
+    ga.load(g + row * D, D, lane);
+    mu_a = mean[row];
+    r_a = rstd[row];
+  }
+  for (; row < rows; row += step) {
+    const float mu = mu_a, r = r_a;
     float xv[NE], gv[NE];
 #pragma unroll
-    for (int c = 0; c < NE / N; ++c) {
-      const int col = chunk_col<LANES, N>(lane, c), cnt = chunk_cnt<N>(D, col);
-      load_vec<T>(xr + col, cnt, xv + c * N);
-      load_vec<T>(gr + col, cnt, gv + c * N);   // zeros behind the row: they add nothing below
+    for (int e = 0; e < NE; ++e) {
+      xv[e] = xa[e];
+      gv[e] = ga[e];
+    }
+    if (row + step < rows) {
+      xa.load(x + (row + step) * D, D, lane);
+      ga.load(g + (row + step) * D, D, lane);
+      mu_a = mean[row + step];
+      r_a = rstd[row + step];
     }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -240,12 +265,12 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void ln_bwd_kernel(
   }
 }
 
-// dw / db = the partial rows added up: 32 columns a workgroup, 8 slices of the partial rows,
+// dw / db = the partial rows added up: 32 columns a workgroup, 32 slices of the partial rows,
 // joined in order.  blockIdx.y: 0 = dw, 1 = db.
 template <typename W>
-__global__ __launch_bounds__(256) void ln_join_kernel(const float* __restrict__ parts, W* dw, W* db,
-                                                      int nparts, int64_t D) {
-  __shared__ float lds[8][32];
+__global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__ parts, W* dw, W* db,
+                                                       int nparts, int64_t D) {
+  __shared__ float lds[32][33];
   W* out = blockIdx.y ? db : dw;
   if (!out) return;
   const int c = threadIdx.x % 32, slice = threadIdx.x / 32;
@@ -253,16 +278,14 @@ __global__ __launch_bounds__(256) void ln_join_kernel(const float* __restrict__ 
   float s = 0.f;
   if (col < D) {
 #pragma unroll 8
-    for (int p = slice; p < nparts; p += 8) s += parts[((int64_t)p * 2 + blockIdx.y) * D + col];
+    for (int p = slice; p < nparts; p += 32) s += parts[((int64_t)p * 2 + blockIdx.y) * D + col];
   }
   lds[slice][c] = s;
   __syncthreads();
-  if (slice == 0 && col < D) {
-    s = lds[0][c];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += lds[k][c];
-    out[col] = (W)s;
-  }
+  // the slices of column `slice`, one a lane
+  s = lane_sum<32>(lds[c][slice]);
+  const int64_t mine = (int64_t)blockIdx.x * 32 + slice;
+  if (c == 0 && mine < D) out[mine] = (W)s;
 }
 
 // ------------------------------------------------ rows too long for a workgroup's registers
@@ -345,69 +368,68 @@ struct Shape {
   int lanes, ne;   // 0: longer than a workgroup keeps
 };
 
-// The fewest lanes and registers that hold a row (N = elements in 16 bytes).
-Shape shape_for(int64_t D, int N) {
+// The fewest lanes that hold a row (N = elements in 16 bytes).  A lane keeps up to 32 elements
+// forward, so that rows of 2048 need no exchange between waves (36064 x 2048 bf16: 68 us); backward
+// keeps five values for each, and 32 of them leave one wave per SIMD (114 us; 16: see below).
+Shape shape_for(int64_t D, int N, bool backward) {
   for (int lanes = 8; lanes <= 64; lanes *= 2)
     if (D <= lanes * N) return {lanes, N};
-  for (int ne = 2 * N; ne <= 32; ne *= 2)
+  for (int ne = 2 * N; ne <= (backward ? 16 : 32); ne *= 2)
     if (D <= 64 * ne) return {64, ne};
-  if (D <= 256 * 16) return {256, 16};
-  if (D <= 256 * 32) return {256, 32};
-  if (D <= 512 * 32) return {512, 32};
+  for (int lanes = 128; lanes <= 1024; lanes *= 2)
+    if (D <= lanes * 16) return {lanes, 16};
   return {0, 0};
 }
 
-int groups_per_block(Shape s) { return s.lanes > 256 ? 1 : 256 / s.lanes; }
+int groups_per_block(Shape s) { return s.lanes > 64 ? 1 : 256 / s.lanes; }
 
-int parts_for(int64_t rows, int64_t D) {
-  // (the larger of the two element widths: enough for either)
-  const Shape a = shape_for(D, 8), b = shape_for(D, 4);
-  const int g = a.lanes && b.lanes ? (groups_per_block(a) < groups_per_block(b) ? groups_per_block(a)
-                                                                               : groups_per_block(b))
-                                   : 1;
+int parts_for(int64_t rows, int64_t D, int N) {
+  const Shape s = shape_for(D, N, true);
+  const int g = s.lanes ? groups_per_block(s) : 1, most = s.lanes ? kMaxParts : 64;
   const int64_t blocks = (rows + g - 1) / g;
-  return (int)(blocks < kMaxParts ? blocks : kMaxParts);
+  return (int)(blocks < most ? blocks : most);
 }
 
-// f(std::integral_constant-like lanes, ne) for the shapes shape_for() gives
+// f(lanes, ne as constants) for the shapes shape_for() gives
 template <int L, int E>
 struct Cfg {
-  static constexpr int lanes = L, ne = E;
+  static constexpr int lanes = L, ne = E, threads = L > 64 ? L : 256, groups = threads / L;
 };
-template <int N, typename F>
+template <int N, bool BACKWARD, typename F>
 int for_shape(Shape s, F f) {
-  if (s.ne == N) {
-    if (s.lanes == 8) return f(Cfg<8, N>());
-    if (s.lanes == 16) return f(Cfg<16, N>());
-    if (s.lanes == 32) return f(Cfg<32, N>());
-    return f(Cfg<64, N>());
+  switch (s.lanes) {
+    case 8: return f(Cfg<8, N>());
+    case 16: return f(Cfg<16, N>());
+    case 32: return f(Cfg<32, N>());
+    case 64:
+      if (s.ne == N) return f(Cfg<64, N>());
+      if (s.ne == 8) return f(Cfg<64, 8>());
+      if (s.ne == 16) return f(Cfg<64, 16>());
+      if constexpr (!BACKWARD) return f(Cfg<64, 32>());
+      return MN_EUNSUPPORTED;
+    case 128: return f(Cfg<128, 16>());
+    case 256: return f(Cfg<256, 16>());
+    case 512: return f(Cfg<512, 16>());
+    default: return f(Cfg<1024, 16>());
   }
-  if (s.lanes == 64) {
-    if (s.ne == 8) return f(Cfg<64, 8>());
-    if (s.ne == 16) return f(Cfg<64, 16>());
-    return f(Cfg<64, 32>());
-  }
-  if (s.lanes == 256) return s.ne == 16 ? f(Cfg<256, 16>()) : f(Cfg<256, 32>());
-  return f(Cfg<512, 32>());
 }
 
 template <typename T, typename W>
 int fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows,
         int64_t D, float eps, hipStream_t st) {
   const float dim = (float)D;
-  const Shape s = shape_for(D, Vec16<T>::N);
+  const Shape s = shape_for(D, Vec16<T>::N, false);
   if (!s.lanes) {
     if (rows >= (1ll << 31)) return MN_EUNSUPPORTED;
     ln_fwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
         (const T*)x, (const W*)w, (const W*)b, (T*)y, mean, rstd, D, dim, eps);
     return mn_launch_status();
   }
-  return for_shape<Vec16<T>::N>(s, [&](auto cfg) {
+  return for_shape<Vec16<T>::N, false>(s, [&](auto cfg) {
     using C = decltype(cfg);
-    constexpr int G = C::lanes > 256 ? 1 : 256 / C::lanes;
-    const int64_t want = (rows + G - 1) / G;
-    const unsigned grid = (unsigned)(want < 2048 ? want : 2048);
-    ln_fwd_kernel<T, W, C::lanes, C::ne><<<grid, C::lanes > 256 ? C::lanes : 256, 0, st>>>(
+        const int64_t want = (rows + C::groups - 1) / C::groups;
+    const unsigned grid = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
+    ln_fwd_kernel<T, W, C::lanes, C::ne><<<grid, C::threads, 0, st>>>(
         (const T*)x, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows, D, dim, eps);
     return mn_launch_status();
   });
@@ -417,7 +439,7 @@ template <typename T, typename W>
 int bwd(const void* g, const void* x, const float* mean, const float* rstd, const void* w, void* dx,
         void* dw, void* db, int64_t rows, int64_t D, float* parts, hipStream_t st) {
   const float dim = (float)D;
-  const Shape s = shape_for(D, Vec16<T>::N);
+  const Shape s = shape_for(D, Vec16<T>::N, true);
   int nparts = 0;
   if (!s.lanes) {
     if (rows >= (1ll << 31) || (D + 255) / 256 >= (1ll << 31)) return MN_EUNSUPPORTED;
@@ -425,20 +447,19 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
       ln_bwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
           (const T*)g, (const T*)x, mean, rstd, (const W*)w, (T*)dx, D, dim);
     if (dw || db) {
-      nparts = parts_for(rows, D) < 64 ? parts_for(rows, D) : 64;
+      nparts = parts_for(rows, D, Vec16<T>::N);
       ln_cols_kernel<T><<<dim3((unsigned)((D + 255) / 256), (unsigned)nparts), 256, 0, st>>>(
           (const T*)g, (const T*)x, mean, rstd, parts, rows, D);
     }
   } else {
-    const int rc = for_shape<Vec16<T>::N>(s, [&](auto cfg) {
+    const int rc = for_shape<Vec16<T>::N, true>(s, [&](auto cfg) {
       using C = decltype(cfg);
-      constexpr int G = C::lanes > 256 ? 1 : 256 / C::lanes;
-      const int64_t want = (rows + G - 1) / G;
-      const int most = parts_for(rows, D);
+            const int64_t want = (rows + C::groups - 1) / C::groups;
+      const int most = parts_for(rows, D, Vec16<T>::N);
       const unsigned grid = (unsigned)(want < most ? want : most);
       const bool join = grid > 1 && (dw || db);
       nparts = join ? (int)grid : 0;
-      ln_bwd_kernel<T, W, C::lanes, C::ne><<<grid, C::lanes > 256 ? C::lanes : 256, 0, st>>>(
+      ln_bwd_kernel<T, W, C::lanes, C::ne><<<grid, C::threads, 0, st>>>(
           (const T*)g, (const T*)x, mean, rstd, (const W*)w, (T*)dx, join ? parts : nullptr,
           join ? nullptr : (W*)dw, join ? nullptr : (W*)db, rows, D, dim);
       return mn_launch_status();
@@ -446,7 +467,7 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
     if (rc != MN_OK) return rc;
   }
   if (nparts)
-    ln_join_kernel<W><<<dim3((unsigned)((D + 31) / 32), 2), 256, 0, st>>>(parts, (W*)dw, (W*)db, nparts, D);
+    ln_join_kernel<W><<<dim3((unsigned)((D + 31) / 32), 2), 1024, 0, st>>>(parts, (W*)dw, (W*)db, nparts, D);
   return mn_launch_status();
 }
 
@@ -483,7 +504,8 @@ int mn_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, floa
 
 size_t mn_layer_norm_ws_bytes(int64_t rows, int64_t D) {
   if (check(rows, D) != MN_OK || rows == 0) return 0;
-  return (size_t)parts_for(rows, D) * 2 * (size_t)D * sizeof(float);
+  const int a = parts_for(rows, D, 4), b = parts_for(rows, D, 8);   // enough for either width
+  return (size_t)(a > b ? a : b) * 2 * (size_t)D * sizeof(float);
 }
 
 int mn_layer_norm_bwd(const void* grad, const void* x, const float* mean, const float* rstd,
