@@ -5,6 +5,8 @@ The reference has no such operator; it follows the contract of its operator clas
 bytes a row, next to BatchNorm's statistics in `params`; the backward needs the stored input.
 fp32, bf16 or fp16; weight and bias have the input's type or fp32.
 """
+import math
+
 import torch
 
 from .. import _lib
@@ -14,12 +16,13 @@ from .base import OP, InputStorage, implements
 def _parameter(t, name, shape, x):
     if t is None:
         return None
-    _lib.require_gpu_tensor(t, name)
-    if tuple(t.shape) != shape:
+    if t.device != x.device:
+        _lib.require_gpu_tensor(t, name)
+        _lib.require_same_device(x, t, name)
+    if t.shape != shape:
         raise RuntimeError(f"{name} must have the normalized shape {list(shape)}, got {list(t.shape)}")
     if t.dtype != x.dtype and t.dtype != torch.float32:
         raise RuntimeError(f"{name} must have dtype {x.dtype} or torch.float32, got {t.dtype}")
-    _lib.require_same_device(x, t, name)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -36,22 +39,18 @@ def layer_norm_forward(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     code = _lib.dtype_code(x, "input")
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     k = len(shape)
-    if k == 0 or tuple(x.shape[x.dim() - k:]) != shape or x.dim() < k:
+    if k == 0 or x.dim() < k or x.shape[x.dim() - k:] != shape:
         raise RuntimeError(f"an input of shape {list(x.shape)} does not end in the normalized shape "
                            f"{list(shape)}")
     w, b = _parameter(weight, "weight", shape, x), _parameter(bias, "bias", shape, x)
     wcode = _lib.DTYPE_CODES[_weight_type(w, b, x)]
     xc = x if x.is_contiguous() else x.contiguous()
-    D = 1
-    for d in shape:
-        D *= d
+    D = math.prod(shape)
     lead = x.shape[:x.dim() - k]
-    rows = 1
-    for d in lead:
-        rows *= d
+    rows = math.prod(lead)
     y = torch.empty_like(xc)
-    mean = torch.empty(lead, dtype=torch.float32, device=x.device)
-    rstd = torch.empty(lead, dtype=torch.float32, device=x.device)
+    mean = x.new_empty(lead, dtype=torch.float32)
+    rstd = x.new_empty(lead, dtype=torch.float32)
     _lib.call_on(x.device, "mn_layer_norm_fwd", xc.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(),
                  mean.data_ptr(), rstd.data_ptr(), rows, D, float(eps), code, wcode)
     return y, mean, rstd
@@ -80,9 +79,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, bias=None, need_input=
     g = grad if grad.is_contiguous() else grad.contiguous()
     mean = mean if mean.is_contiguous() else mean.contiguous()
     rstd = rstd if rstd.is_contiguous() else rstd.contiguous()
-    D = 1
-    for d in shape:
-        D *= d
+    D = math.prod(shape)
     rows = mean.numel()
     dx = torch.empty_like(xc) if need_input else None
     dw = None if w is None else torch.empty(shape, dtype=wtype, device=x.device)
