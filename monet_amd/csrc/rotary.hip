@@ -19,6 +19,8 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kSlots = 4;
+constexpr int kBlockElems = 4096;
 constexpr int kMaxPairs = 128;
 constexpr int64_t kMaxToken = 1 << 24;   // elements of a token
 constexpr int kTableFloats = 8192;   // 32 KB of LDS: TOK * pairs * 2
@@ -64,54 +66,81 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const T* __restrict__ 
     table[i] = cs;
   }
   __syncthreads();
-  // units of a head: chunks of pairs (N pairs, or N / 2 interleaved), then chunks that are copied
-  const int per = INTERLEAVED ? N / 2 : N;
-  const int pair_units = (a.n + per - 1) / per, rest = a.D - 2 * a.n;
-  const int units = pair_units + (rest + N - 1) / N;
-  const uint32_t per_token = (uint32_t)a.H * units;
-  const uint32_t total = (uint32_t)batches * toks * per_token;
-  for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
-    const uint32_t bt = i / per_token, hu = i - bt * per_token;
-    const int h = hu / units, u = hu - h * units;
-    const uint32_t bi = bt / toks;
-    const int t = bt - bi * toks;
-    const int64_t b = b0 + bi;
-    const T* xr = x + b * a.sxb + (t0 + t) * a.sxt + h * a.sxh;
-    T* yr = y + ((b * a.T + t0 + t) * a.H + h) * a.D;
-    if (u >= pair_units) {
-      const int col = 2 * a.n + (u - pair_units) * N;
-      const int cnt = a.D - col < N ? a.D - col : N;
-      float v[N];
-      load_vec<T>(xr + col, cnt, v);
-      store_vec<T>(yr + col, cnt, v);
-      continue;
+  // Units of a head: chunks of N pairs, then chunks that are copied; interleaved, chunks of N
+  // elements, where what is copied is a pair that turns by nothing (so that only the end of a head
+  // is less than 16 bytes).
+  // A wave takes a token at a time, a lane the same kSlots units of each, so that what a unit is
+  // and where it lies is worked out once; tokens of at most 64 units are taken kSlots at a time.
+  // All loads of a turn are on their way before the first is used.
+  const int pair_units = INTERLEAVED ? (a.D + N - 1) / N : (a.n + N - 1) / N;
+  const int units = INTERLEAVED ? pair_units : pair_units + (a.D - 2 * a.n + N - 1) / N, per_token = a.H * units;
+  const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE, waves = kThreads / MN_WAVE;
+  const bool narrow = per_token <= MN_WAVE;
+  const int tokens = batches * toks, step = narrow ? waves * kSlots : waves;
+  for (int first = 0; first < per_token; first += narrow ? MN_WAVE : MN_WAVE * kSlots) {
+    int64_t xo[kSlots];
+    int yo[kSlots], tab[kSlots], cnt[kSlots];   // cnt: elements (of either half of the pairs); 0: nothing
+    bool copy[kSlots];
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+      const int hu = first + (narrow ? 0 : k * MN_WAVE) + lane;
+      const int h = hu / units, u = hu - h * units;
+      copy[k] = !INTERLEAVED && u >= pair_units;
+      const int col = copy[k] ? 2 * a.n + (u - pair_units) * N : u * N;
+      xo[k] = h * a.sxh + col;
+      yo[k] = h * a.D + col;
+      tab[k] = INTERLEAVED ? col / 2 : col;   // first pair
+      const int left = (INTERLEAVED || copy[k] ? a.D : a.n) - col;
+      cnt[k] = hu < per_token ? (left < N ? left : N) : 0;
     }
-    const int p0 = u * per, pairs = a.n - p0 < per ? a.n - p0 : per;
-    const float2_t* cs = table + t * a.n + p0;
-    float v[N], w[N];
-    if (INTERLEAVED) {
-      load_vec<T>(xr + 2 * p0, 2 * pairs, v);
+    for (int bt0 = wave; bt0 < tokens; bt0 += step) {
+      typename Vec16<T>::type lo[kSlots], hi[kSlots];
 #pragma unroll
-      for (int e = 0; e < N / 2; ++e) {
-        if (e >= pairs) break;
-        const float2_t c = cs[e];
-        w[2 * e] = v[2 * e] * c[0] - v[2 * e + 1] * c[1];
-        w[2 * e + 1] = v[2 * e] * c[1] + v[2 * e + 1] * c[0];
+      for (int k = 0; k < kSlots; ++k) {
+        const int bt = bt0 + (narrow ? k * waves : 0);
+        if (bt >= tokens || cnt[k] == 0) continue;
+        const int bi = bt / toks, t = bt - bi * toks;
+        const T* p = x + (b0 + bi) * a.sxb + (t0 + t) * a.sxt + xo[k];
+        lo[k] = load_raw<T>(p, cnt[k]);
+        if (!INTERLEAVED && !copy[k]) hi[k] = load_raw<T>(p + a.n, cnt[k]);
       }
-      store_vec<T>(yr + 2 * p0, 2 * pairs, w);
-    } else {
-      load_vec<T>(xr + p0, pairs, v);
-      load_vec<T>(xr + a.n + p0, pairs, w);
-      float lo[N], hi[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (e >= pairs) break;
-        const float2_t c = cs[e];
-        lo[e] = v[e] * c[0] - w[e] * c[1];
-        hi[e] = v[e] * c[1] + w[e] * c[0];
+      for (int k = 0; k < kSlots; ++k) {
+        const int bt = bt0 + (narrow ? k * waves : 0);
+        if (bt >= tokens || cnt[k] == 0) continue;
+        const int bi = bt / toks, t = bt - bi * toks;
+        T* q = y + ((b0 + bi) * a.T + t0 + t) * (int64_t)(a.H * a.D) + yo[k];
+        float v[N];
+        if (copy[k]) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = (float)lo[k][e];
+          store_vec<T>(q, cnt[k], v);
+          continue;
+        }
+        const float2_t* cs = table + t * a.n + tab[k];
+        if (INTERLEAVED) {
+#pragma unroll
+          for (int e = 0; e < N / 2; ++e) {
+            const bool turns = tab[k] + e < a.n;
+            const float2_t c = turns ? cs[e] : float2_t{1.f, 0.f};
+            const float f = (float)lo[k][2 * e], g = (float)lo[k][2 * e + 1];
+            v[2 * e] = turns ? f * c[0] - g * c[1] : f;   // (a copied infinity is no pair's)
+            v[2 * e + 1] = turns ? f * c[1] + g * c[0] : g;
+          }
+          store_vec<T>(q, cnt[k], v);
+        } else {
+          float w[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float2_t c = cs[e < cnt[k] ? e : 0];
+            const float f = (float)lo[k][e], g = (float)hi[k][e];
+            v[e] = f * c[0] - g * c[1];
+            w[e] = f * c[1] + g * c[0];
+          }
+          store_vec<T>(q, cnt[k], v);
+          store_vec<T>(q + a.n, cnt[k], w);
+        }
       }
-      store_vec<T>(yr + p0, pairs, lo);
-      store_vec<T>(yr + a.n + p0, pairs, hi);
     }
   }
 }
@@ -146,10 +175,10 @@ int mn_rotary(const mn_rotary_desc* d, const void* x, const void* positions, voi
   a.sxb = d->x_stride[0]; a.sxt = d->x_stride[1]; a.sxh = d->x_stride[2];
   a.spa = d->pos_stride[0]; a.spb = d->pos_stride[1]; a.spt = d->pos_stride[2];
   a.sign = inverse ? -1.f : 1.f;
-  // tokens of a workgroup: about 16 KB of x in all, as far as the table has room; entries of the
+  // tokens of a workgroup: about kBlockElems elements of x, as far as the table has room; entries of the
   // batch share the table unless their positions differ, as long as 2048 workgroups remain
   const int64_t token_elems = (int64_t)a.H * a.D;
-  int64_t tok = token_elems ? 8192 / token_elems : 1;
+  int64_t tok = token_elems ? kBlockElems / token_elems : 1;
   const int64_t room = n ? kTableFloats / (2 * n) : 64;
   tok = tok < 1 ? 1 : (tok > room ? room : (tok > 64 ? 64 : tok));
   if (tok > a.T) tok = a.T > 0 ? a.T : 1;
