@@ -21,6 +21,8 @@
 // chunk c ^ swz(r), which spreads both kinds of reads over all banks: rows (a lane reads 16 bytes
 // of its row) and transposed (16-bit: ds_read_b64_tr_b16 gives a lane four rows' values of its
 // column; fp32: plain 4-byte reads).
+#include <type_traits>
+
 #include "elem.h"
 
 namespace {
@@ -127,13 +129,12 @@ struct Tile {
     return (row * NC + (chunk ^ swz(row))) * 16;
   }
 
-  // global -> registers: rows r0 .. r0 + ROWS of a head, rows from `end` on as zeros
-  static __device__ __forceinline__ void fetch(frag* regs, const T* base, int64_t stride, int r0, int end,
-                                               int D) {
+  // global -> registers: the tile's rows from `rows` on, zeros from row `left` on
+  static __device__ __forceinline__ void fetch(frag* regs, const T* rows, int64_t stride, int left, int D) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-      const int idx = threadIdx.x + p * kThreads, row = r0 + idx / CH, col = idx % CH * N;
-      regs[p] = chunk(base + row * stride + col, row < end ? D - col : 0);
+      const int idx = threadIdx.x + p * kThreads, row = idx / CH, col = idx % CH * N;
+      regs[p] = chunk(rows + row * stride + col, row < left ? D - col : 0);
     }
   }
   static __device__ __forceinline__ frag chunk(const T* p, int cnt) {
@@ -167,13 +168,22 @@ struct Tile {
   // `offsets`: those of a whole tile, which a thread keeps
   static __device__ __forceinline__ void load(uint32_t lds, const T* rows, const uint32_t* offsets, int64_t stride,
                                               int left, int D) {
+    if (__builtin_expect(left < ROWS, 0)) {
+      asm volatile("");   // (a branch, not both sides)
+      uint32_t cut[SLOTS];
+#pragma unroll
+      for (int p = 0; p < SLOTS; ++p) cut[p] = offset(p, left, stride);
+      load_all(lds, rows, cut, D);
+    } else {
+      load_all(lds, rows, offsets, D);
+    }
+  }
+  static __device__ __forceinline__ void load_all(uint32_t lds, const T* rows, const uint32_t* offsets, int D) {
 #pragma unroll
     for (int p = 0; p < SLOTS; ++p) {
       const int slot = threadIdx.x + p * kThreads, chunk = slot % NC ^ swz(slot / NC);
       const uint32_t at = lds + (p * kThreads + (threadIdx.x & ~(MN_WAVE - 1))) * 16;
-      uint32_t off = offsets[p];
-      if (left < ROWS) off = offset(p, left, stride);
-      if (D == NC * N || chunk * N < D) load_to_lds((const char*)rows, off, at);
+      if (D == NC * N || chunk * N < D) load_to_lds((const char*)rows, offsets[p], at);
     }
   }
   static __device__ __forceinline__ void clear(char* lds, int D) {
@@ -242,16 +252,15 @@ struct Stage {
       }
     }
   }
-  // tile n: rows row0 .. of two heads
-  __device__ __forceinline__ void begin(int n, const T* a, int64_t sa, const T* b, int64_t sb, int row0,
-                                        int end, int D) {
+  // tile n: rows of two heads from a and b on, `left` of them there
+  __device__ __forceinline__ void begin(int n, const T* a, int64_t sa, const T* b, int64_t sb, int left, int D) {
     if constexpr (DIRECT) {
       const uint32_t at = lds_address(buffer(n));
-      Ti::load(at, a + row0 * sa, o0, sa, end - row0, D);
-      Ti::load(at + Ti::BYTES, b + row0 * sb, o1, sb, end - row0, D);
+      Ti::load(at, a, o0, sa, left, D);
+      Ti::load(at + Ti::BYTES, b, o1, sb, left, D);
     } else {
-      Ti::fetch(r0, a, sa, row0, end, D);
-      Ti::fetch(r1, b, sb, row0, end, D);
+      Ti::fetch(r0, a, sa, left, D);
+      Ti::fetch(r1, b, sb, left, D);
     }
   }
   __device__ __forceinline__ void finish(int n) {
@@ -421,13 +430,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
     const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
     Stage<T, DP, R, DIRECT, 0> stage;
     stage.init(lds, a.sk[1], a.sv[1], a.D);
-    stage.begin(0, kb, a.sk[1], vb, a.sv[1], kt.tile(0) * R, len, a.D);
+    const auto begin = [&](int n) {
+      const int row0 = kt.tile(n) * R;
+      stage.begin(n, kb + row0 * a.sk[1], a.sk[1], vb + row0 * a.sv[1], a.sv[1], len - row0, a.D);
+    };
+    begin(0);
     for (int n = 0; n < n_tiles; ++n) {
       const char* kl = stage.buffer(n);
       const char* vl = kl + Ti::BYTES;
       stage.finish(n);
       __syncthreads();   // (everyone is done with the other buffer)
-      if (n + 1 < n_tiles) stage.begin(n + 1, kb, a.sk[1], vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
+      if (n + 1 < n_tiles) begin(n + 1);
       const int j0 = kt.tile(n) * R;
       if (w0 >= len || none_visible(a, w0, w1, j0, j0 + R - 1)) continue;
       f32x16 s[KT];
@@ -451,7 +464,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
       top = max_xor32(top) * a.scale_log2;
       // a new maximum only where the old one is left behind by more than 2^8: below that P stays
       // below 2^8 and nothing has to be scaled
-      if (__any(top > m + 8.f)) {
+      if (__builtin_expect(__any(top > m + 8.f), 0)) {
         const float now = fmaxf(m, top), f = now == -INFINITY ? 1.f : exp2f(m - now);
         m = now;
         sum *= f;
@@ -522,13 +535,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
     const int n_tiles = kt.count(), w1 = min(w0 + 31, len - 1);
     Stage<T, DP, R, DIRECT, 0> stage;
     stage.init(lds, a.sk[1], a.sv[1], a.D);
-    stage.begin(0, kb, a.sk[1], vb, a.sv[1], kt.tile(0) * R, len, a.D);
+    const auto begin = [&](int n) {
+      const int row0 = kt.tile(n) * R;
+      stage.begin(n, kb + row0 * a.sk[1], a.sk[1], vb + row0 * a.sv[1], a.sv[1], len - row0, a.D);
+    };
+    begin(0);
     for (int n = 0; n < n_tiles; ++n) {
       const char* kl = stage.buffer(n);
       const char* vl = kl + Ti::BYTES;
       stage.finish(n);
       __syncthreads();
-      if (n + 1 < n_tiles) stage.begin(n + 1, kb, a.sk[1], vb, a.sv[1], kt.tile(n + 1) * R, len, a.D);
+      if (n + 1 < n_tiles) begin(n + 1);
       const int j0 = kt.tile(n) * R;
       if (w0 >= len) continue;
 #pragma unroll
@@ -622,27 +639,41 @@ struct QueryTiles {
   St stage;
   int count, row;                   // tiles; first row of the one that was finished last
   int first, head, next, pending;   // what begin() will load, what it has begun
+  const T *qp, *gp;                 // rows `next` of head `head`
+  const float *lp, *dp;
   float lreg = 0.f, dreg = 0.f;
+  __device__ __forceinline__ void point(const Args& a, const KeyWork& w) {
+    qp = (const T*)a.q + w.b * a.sq[0] + head * a.sq[2] + next * a.sq[1];
+    gp = (const T*)a.grad + (((int64_t)w.b * a.T + next) * a.Hq + head) * a.D;
+    const int64_t stat = ((int64_t)w.b * a.Hq + head) * a.T + next;
+    lp = a.lse + stat;
+    dp = a.delta + stat;
+  }
   __device__ __forceinline__ void init(const Args& a, const KeyWork& w, char* lds) {
     first = next = w.lo / R * R;
     count = (w.hi / R + 1 - w.lo / R) * a.group;
     head = w.hk * a.group;
     stage.init(lds, a.sq[1], (int64_t)a.Hq * a.D, a.D);
+    point(a, w);
   }
   __device__ __forceinline__ void begin(const Args& a, const KeyWork& w, int n) {
     pending = next;
-    stage.begin(n, (const T*)a.q + w.b * a.sq[0] + head * a.sq[2], a.sq[1],
-                (const T*)a.grad + ((int64_t)w.b * a.T * a.Hq + head) * a.D, (int64_t)a.Hq * a.D, next, w.len, a.D);
+    stage.begin(n, qp, a.sq[1], gp, (int64_t)a.Hq * a.D, w.len - next, a.D);
     if (threadIdx.x < R) {
-      const int i = next + threadIdx.x;
-      const int64_t stat = ((int64_t)w.b * a.Hq + head) * a.T + i;
-      lreg = i < w.len ? a.lse[stat] : INFINITY;   // no query: P = exp2(-inf) = 0
-      dreg = i < w.len ? a.delta[stat] : 0.f;
+      const bool there = next + (int)threadIdx.x < w.len;
+      lreg = there ? lp[threadIdx.x] : INFINITY;   // no query: P = exp2(-inf) = 0
+      dreg = there ? dp[threadIdx.x] : 0.f;
     }
     next += R;
     if (next > w.hi) {
       next = first;
       ++head;
+      point(a, w);
+    } else {
+      qp += R * a.sq[1];
+      gp += (int64_t)R * a.Hq * a.D;
+      lp += R;
+      dp += R;
     }
   }
   __device__ __forceinline__ const char* q(int n) const { return stage.buffer(n); }
@@ -673,64 +704,69 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void 
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) acc[d] = (f32x16)(0.f);
   if (w.k0 < w.len && w.lo <= w.hi) {
-    frag kf[Ti::STEPS], vf[Ti::STEPS];
-    own_row<T, DP>(kf, (const T*)a.k + w.b * a.sk[0] + w.hk * a.sk[2] + j * a.sk[1], j < w.len, a.D);
-    own_row<T, DP>(vf, (const T*)a.v + w.b * a.sv[0] + w.hk * a.sv[2] + j * a.sv[1], j < w.len, a.D);
     QueryTiles<T, DP, R, DIRECT> tiles;
     tiles.init(a, w, lds);
     tiles.begin(a, w, 0);
-    for (int n = 0; n < tiles.count; ++n) {
-      const char *ql = tiles.q(n), *gl = tiles.g(n);
-      const float* stats = tiles.stats(n);
-      tiles.finish(n);
-      __syncthreads();
-      const int row0 = tiles.row;
-      if (n + 1 < tiles.count) tiles.begin(a, w, n + 1);
+    frag kf[Ti::STEPS];
+    own_row<T, DP>(kf, (const T*)a.k + w.b * a.sk[0] + w.hk * a.sk[2] + j * a.sk[1], j < w.len, a.D);
+    const auto walk = [&](auto which) {
+      constexpr bool DK = decltype(which)::value;
+      frag vf[DK ? Ti::STEPS : 1];
+      if constexpr (DK)
+        own_row<T, DP>(vf, (const T*)a.v + w.b * a.sv[0] + w.hk * a.sv[2] + j * a.sv[1], j < w.len, a.D);
+      for (int n = 0; n < tiles.count; ++n) {
+        const char *ql = tiles.q(n), *gl = tiles.g(n);
+        const float* stats = tiles.stats(n);
+        tiles.finish(n);
+        __syncthreads();
+        const int row0 = tiles.row;
+        if (n + 1 < tiles.count) tiles.begin(a, w, n + 1);
 #pragma unroll
-      for (int t = 0; t < R / 32; ++t) {
-        const int it = row0 + t * 32;
-        // (queries outside [lo, hi] belong to another workgroup of the tile)
-        if (w0 >= w.len || it > w.hi || it + 31 < w.lo || none_visible(a, it, it + 31, w0, w1)) continue;
-        f32x16 s = (f32x16)(0.f);
+        for (int t = 0; t < R / 32; ++t) {
+          const int it = row0 + t * 32;
+          // (queries outside [lo, hi] belong to another workgroup of the tile)
+          if (w0 >= w.len || it > w.hi || it + 31 < w.lo || none_visible(a, it, it + 31, w0, w1)) continue;
+          f32x16 s = (f32x16)(0.f), p = (f32x16)(0.f);
 #pragma unroll
-        for (int st = 0; st < Ti::STEPS; ++st) s = Mma<T>::mul(Ti::rows(ql, t * 32, st), kf[st], s);
-        if constexpr (sizeof(T) == 2) feed<Ti::STEPS, 1, 4 < Ti::STEPS ? 4 : Ti::STEPS>();
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4_t l2 = *reinterpret_cast<const float4_t*>(stats + t * 32 + g * 8 + lane / 32 * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale_log2, -l2[e]));
-        }
-        if (w.is_dk) {
-          f32x16 p = (f32x16)(0.f);
-#pragma unroll
-          for (int st = 0; st < Ti::STEPS; ++st) p = Mma<T>::mul(Ti::rows(gl, t * 32, st), vf[st], p);
-          if constexpr (sizeof(T) == 2) feed<Ti::STEPS, 1, 4 < Ti::STEPS ? 4 : Ti::STEPS>();
+          for (int st = 0; st < Ti::STEPS; ++st) {
+            s = Mma<T>::mul(Ti::rows(ql, t * 32, st), kf[st], s);
+            if constexpr (DK) p = Mma<T>::mul(Ti::rows(gl, t * 32, st), vf[st], p);
+          }
+          if constexpr (sizeof(T) == 2) feed<(DK ? 2 : 1) * Ti::STEPS, 1, DK ? 4 : (Ti::STEPS < 4 ? Ti::STEPS : 4)>();
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const float4_t de = *reinterpret_cast<const float4_t*>(stats + R + t * 32 + g * 8 + lane / 32 * 4);
+            const float4_t l2 = *reinterpret_cast<const float4_t*>(stats + t * 32 + g * 8 + lane / 32 * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] *= p[4 * g + e] - de[e];
+            for (int e = 0; e < 4; ++e)
+              s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale_log2, -l2[e]));
+            if constexpr (DK) {
+              const float4_t de = *reinterpret_cast<const float4_t*>(stats + R + t * 32 + g * 8 + lane / 32 * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[4 * g + e] *= p[4 * g + e] - de[e];
+            }
           }
-        }
-        if (!(it >= w.lo && it + 31 <= w.hi && all_visible(a, it, it + 31, w0, w0 + 31, w.len))) {
-          keep_branch();
-          const int last = j < a.sinks ? w.hi : min(w.hi, j + a.left);
-          const Seen see = interval(max(w.lo, j - a.right), j < w.len ? last : -1, 0, it);
+          if (!(it >= w.lo && it + 31 <= w.hi && all_visible(a, it, it + 31, w0, w0 + 31, w.len))) {
+            keep_branch();
+            const int last = j < a.sinks ? w.hi : min(w.hi, j + a.left);
+            const Seen see = interval(max(w.lo, j - a.right), j < w.len ? last : -1, 0, it);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = see(acc_row(r)) ? s[r] : 0.f;
-        }
-        const char* rows = w.is_dk ? ql : gl;
+            for (int r = 0; r < 16; ++r) s[r] = see(acc_row(r)) ? s[r] : 0.f;
+          }
 #pragma unroll
-        for (int st = 0; st < Acc<T>::STEPS; ++st) {
-          const frag f = Acc<T>::operand(s, st);
+          for (int st = 0; st < Acc<T>::STEPS; ++st) {
+            const frag f = Acc<T>::operand(s, st);
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::mul(Ti::cols(rows, t * 32, st, d * 32), f, acc[d]);
+            for (int d = 0; d < DP / 32; ++d)
+              acc[d] = Mma<T>::mul(Ti::cols(DK ? ql : gl, t * 32, st, d * 32), f, acc[d]);
+          }
+          if constexpr (sizeof(T) == 2) feed<Acc<T>::STEPS * DP / 32, 2, 2>();
         }
-        if constexpr (sizeof(T) == 2) feed<Acc<T>::STEPS * DP / 32, 2, 2>();
       }
-    }
+    };
+    if (w.is_dk)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
   }
   if (j >= a.T) return;
   const float factor = w.is_dk ? a.scale : 1.f;
