@@ -21,6 +21,7 @@
 // chunk c ^ swz(r), which spreads both kinds of reads over all banks: rows (a lane reads 16 bytes
 // of its row) and transposed (16-bit: ds_read_b64_tr_b16 gives a lane four rows' values of its
 // column; fp32: plain 4-byte reads).
+#include <mutex>
 #include <type_traits>
 
 #include "elem.h"
@@ -134,19 +135,28 @@ struct Tile {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int idx = threadIdx.x + p * kThreads, row = idx / CH, col = idx % CH * N;
-      regs[p] = chunk(rows + row * stride + col, row < left ? D - col : 0);
+      regs[p] = chunk(rows + row * stride + col, row < left ? D - col : 0, D);
     }
   }
-  static __device__ __forceinline__ frag chunk(const T* p, int cnt) {
-    frag f;
-    if (cnt >= N) {
-      const typename Vec16<T>::utype v = *reinterpret_cast<const typename Vec16<T>::utype*>(p);
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = e < cnt ? p[e] : (T)0.f;
+  // `cnt` elements of a row from p on, zeros behind them.  The end of a row of at least N elements
+  // is taken from the 16 bytes that end there, moved down: one load, no loop over elements.
+  static __device__ __forceinline__ frag chunk(const T* p, int cnt, int D) {
+    if (cnt <= 0) return (frag)(0.f);
+    if (D >= N) {
+      const int missing = max(N - cnt, 0);
+      typedef uint64_t half2 __attribute__((ext_vector_type(2)));
+      half2 v = __builtin_bit_cast(half2, *reinterpret_cast<const typename Vec16<T>::utype*>(p - missing));
+      if (missing) {
+        const int bits = missing * 8 * (int)sizeof(T);   // 16 .. 112
+        const uint64_t lo = bits < 64 ? v[0] >> bits | v[1] << (64 - bits) : v[1] >> (bits - 64);
+        v[1] = bits < 64 ? v[1] >> bits : 0;
+        v[0] = lo;
+      }
+      return __builtin_bit_cast(frag, v);
     }
+    frag f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = e < cnt ? p[e] : (T)0.f;
     return f;
   }
   static __device__ __forceinline__ void put(char* lds, const frag* regs) {
@@ -350,7 +360,7 @@ __device__ __forceinline__ void own_row(typename Mma<T>::frag* f, const T* row, 
 #pragma unroll
   for (int s = 0; s < Ti::STEPS; ++s) {
     const int col = (2 * s + half) * Ti::N;
-    f[s] = Ti::chunk(row + col, valid ? D - col : 0);
+    f[s] = Ti::chunk(row + col, valid ? D - col : 0, D);
   }
 }
 
@@ -398,6 +408,9 @@ __device__ __forceinline__ TileOf tile_of(const Args& a, int tiles, bool last_is
   return {last_is_long ? tiles - 1 - from_front : from_front, (int)(slot / tiles)};
 }
 
+// What the registers allow (fp32 at D > 64: operands and accumulators need more than 256).
+template <typename T, int DP>
+constexpr int kWavesPerSimd = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
 // Rows of keys in a tile: fp32 rows are twice as long.
 template <typename T>
 constexpr int kRows = sizeof(T) == 2 ? 64 : 32;
@@ -405,7 +418,7 @@ constexpr int kQueries = 32 * kWaves;   // queries (or, for dk / dv, keys) of a 
 
 // --------------------------------------------------------------------------------- forward
 template <typename T, int DP, bool DIRECT>
-__global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_fwd_kernel(const Args a) {
   constexpr int R = kRows<T>, KT = R / 32;
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
@@ -501,7 +514,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(const Args a) {
 
 // -------------------------------------------------------------- backward: dq (and rowsum(do o))
 template <typename T, int DP, bool DIRECT>
-__global__ __launch_bounds__(kThreads, 2) void attn_dq_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_dq_kernel(const Args a) {
   constexpr int R = kRows<T>, KT = R / 32;
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
@@ -692,7 +705,7 @@ struct QueryTiles {
 };
 
 template <typename T, int DP, bool DIRECT>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attn_dkv_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_dkv_kernel(const Args a) {
   constexpr int R = kRows<T>;
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
@@ -807,9 +820,9 @@ int check(const mn_attention* d) {
   if (d->Hq % d->Hkv || d->left < -1 || d->right < -1 || d->sinks < 0) return MN_EINVAL;
   if (!(d->scale > 0.f) || d->scale > 1e30f) return MN_EINVAL;
   if (d->D > kMaxD || d->T >= (1 << 28)) return MN_EUNSUPPORTED;
-  // one workgroup per tile, head and entry, counted in 32 bits (dk / dv: at most twice the tiles)
+  // one workgroup per tile, head and entry, counted in 31 bits (dk and dv: at most six times that)
   const int64_t tiles = (d->T + kQueries - 1) / kQueries;
-  if (d->B >= (1 << 28) || d->Hq >= (1 << 20) || (tiles && d->B * d->Hq > (1ll << 30) / tiles))
+  if (d->B >= (1 << 28) || d->Hq >= (1 << 20) || (tiles && d->B * d->Hq > (1ll << 28) / tiles))
     return MN_EUNSUPPORTED;
   return MN_OK;
 }
@@ -819,17 +832,20 @@ int32_t limit(int64_t v, int64_t T) { return (int32_t)(v < 0 || v > T ? T : v); 
 
 // How the queries behind the window of the key tiles with sinks are cut: chunks that make 1024
 // rows to walk over (all heads of the group), longer ones where that would be more than 128
-// chunks.  Shorter ones start and end more often than they multiply (115 chunks of 128 queries at
-// T = 15808, 16 heads of keys: 2.7 ms against 1.9), much longer ones outlast a plain tile.  Not
-// cut where the sinks are more than an eighth of the keys (enough workgroups share the walk then).
+// chunks, or more than two for each plain tile.  Shorter ones start and end more often than they
+// multiply (T = 15808, four batches of 16 heads: 2.70 ms in chunks of 128, 2.32 of 1024), much
+// longer ones outlast a plain tile.  Not cut where the sinks are more than an eighth of the keys
+// (enough workgroups share the walk then).
 void split_for(const mn_attention* d, Args* a) {
   a->sink_tiles = a->nchunks = 0;
   a->chunk = 1;
-  const int64_t T = d->T, left = limit(d->left, T);
+  const int64_t T = d->T, left = limit(d->left, T), all = (T + kQueries - 1) / kQueries;
   const int64_t sinks = d->sinks < T ? d->sinks : T, tiles = (sinks + kQueries - 1) / kQueries;
   const int64_t behind = T - kQueries - left;   // queries behind the window of the first tile
   if (sinks == 0 || behind <= 0 || tiles * kQueries * 8 > T) return;
-  int64_t chunk = (behind + 127) / 128;
+  int64_t most = 2 * all / tiles;               // at least 16
+  if (most > 128) most = 128;
+  int64_t chunk = (behind + most - 1) / most;
   const int64_t rows = 1024 / (d->Hq / d->Hkv);
   chunk = chunk < rows ? rows : chunk;
   chunk = (chunk + 63) / 64 * 64;
@@ -882,35 +898,37 @@ bool direct_rows(const void* p, const int64_t* stride, const mn_attention* d, in
          stride[2] % n == 0 && stride[1] >= 0 && stride[1] < (1 << 22);   // 64 rows in 31 bits
 }
 
-// Dynamic LDS of more than 64 KB has to be asked for, once per kernel and device.
-template <typename K>
-bool raise_lds(K kernel, int bytes) {
-  return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
-}
-
 template <typename T, int DP>
 constexpr int kLdsQ = 4 * Tile<T, DP, kRows<T>>::BYTES;   // two buffers of two tiles
 template <typename T, int DP>
 constexpr int kLdsKv = kLdsQ<T, DP> + 4 * kRows<T> * (int)sizeof(float);   // and two rows' statistics
 
+// Dynamic LDS of more than 64 KB (dk / dv at D > 64) has to be asked for.
 template <typename T, int DP, bool DIRECT>
-bool init_one() {
-  return raise_lds(attn_fwd_kernel<T, DP, DIRECT>, kLdsQ<T, DP>) && raise_lds(attn_dq_kernel<T, DP, DIRECT>, kLdsQ<T, DP>) &&
-         raise_lds(attn_dkv_kernel<T, DP, DIRECT>, kLdsKv<T, DP>);
+bool raise_lds() {
+  static_assert(kLdsQ<T, DP> <= 65536, "only dk / dv need more");
+  return kLdsKv<T, DP> <= 65536 ||
+         hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_dkv_kernel<T, DP, DIRECT>),
+                             hipFuncAttributeMaxDynamicSharedMemorySize, kLdsKv<T, DP>) == hipSuccess;
 }
 template <typename T>
-bool init_type() {
-  return init_one<T, 32, false>() && init_one<T, 64, false>() && init_one<T, 96, false>() &&
-         init_one<T, 128, false>() && init_one<T, 32, true>() && init_one<T, 64, true>() &&
-         init_one<T, 96, true>() && init_one<T, 128, true>();
+bool raise_lds_of() {
+  return raise_lds<T, 64, false>() && raise_lds<T, 96, false>() && raise_lds<T, 128, false>() &&
+         raise_lds<T, 64, true>() && raise_lds<T, 96, true>() && raise_lds<T, 128, true>();
 }
 
 }  // namespace
 
-// The limits of dynamic LDS, which are not a stream operation: from mn_init, and again from the
-// entry points (a caller that never calls mn_init).
-bool mn_attention_init() { return init_type<float>() && init_type<bf16_t>() && init_type<f16_t>(); }
+// Once per device: from mn_init, or from the first backward pass of a caller that never calls it.
+bool mn_attention_init() {
+  static std::mutex lock;
+  static bool done[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+  std::lock_guard<std::mutex> hold(lock);
+  if (!done[dev]) done[dev] = raise_lds_of<float>() && raise_lds_of<bf16_t>() && raise_lds_of<f16_t>();
+  return done[dev];
+}
 
 extern "C" {
 
@@ -929,7 +947,6 @@ int mn_attention_fwd(const mn_attention* d, const void* q, const void* k, const 
     return for_width(d->D, direct, [&](auto w) {
       constexpr int DP = decltype(w)::value, lds = kLdsQ<T, DP>;
       constexpr bool DIRECT = decltype(w)::direct;
-      if (!raise_lds(attn_fwd_kernel<T, DP, DIRECT>, lds)) return (int)MN_ELAUNCH;
       attn_fwd_kernel<T, DP, DIRECT><<<grid, kThreads, lds, mn_stream(stream)>>>(a);
       return mn_launch_status();
     });
@@ -966,8 +983,7 @@ int mn_attention_bwd(const mn_attention* d, const void* grad, const void* q, con
     const int rc = for_width(d->D, direct, [&](auto w) {
       constexpr bool DIRECT = decltype(w)::direct;
       constexpr int DP = decltype(w)::value, lds_q = kLdsQ<T, DP>, lds_kv = kLdsKv<T, DP>;
-      if (!raise_lds(attn_dq_kernel<T, DP, DIRECT>, lds_q) || !raise_lds(attn_dkv_kernel<T, DP, DIRECT>, lds_kv))
-        return (int)MN_ELAUNCH;
+      if (lds_kv > 65536 && !mn_attention_init()) return (int)MN_ELAUNCH;
       attn_dq_kernel<T, DP, DIRECT><<<(unsigned)(a.tiles * d->Hq * d->B), kThreads, lds_q, s>>>(a);
       const unsigned items = (unsigned)(a.tiles + a.sink_tiles * a.nchunks);
       attn_dkv_kernel<T, DP, DIRECT><<<(unsigned)(2 * items * d->Hkv * d->B), kThreads, lds_kv, s>>>(a);

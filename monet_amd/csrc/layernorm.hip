@@ -443,14 +443,15 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
   int nparts = 0;
   if (!s.lanes) {
     if (rows >= (1ll << 31) || (D + 255) / 256 >= (1ll << 31)) return MN_EUNSUPPORTED;
-    if (dx)
-      ln_bwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
-          (const T*)g, (const T*)x, mean, rstd, (const W*)w, (T*)dx, D, dim);
+    // (before dx, which may take the gradient's place)
     if (dw || db) {
       nparts = parts_for(rows, D, Vec16<T>::N);
       ln_cols_kernel<T><<<dim3((unsigned)((D + 255) / 256), (unsigned)nparts), 256, 0, st>>>(
           (const T*)g, (const T*)x, mean, rstd, parts, rows, D);
     }
+    if (dx)
+      ln_bwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
+          (const T*)g, (const T*)x, mean, rstd, (const W*)w, (T*)dx, D, dim);
   } else {
     const int rc = for_shape<Vec16<T>::N, true>(s, [&](auto cfg) {
       using C = decltype(cfg);

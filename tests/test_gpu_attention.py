@@ -149,7 +149,8 @@ def test_shared_heads(cuda, H, K, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T,left,right,sinks", [(1100, 60, 0, 1), (1500, 100, 0, 3), (2600, 64, 10, 200),
-                                                (3000, 1, 0, 128), (2049, 0, 0, 129), (1300, 500, 0, 4)])
+                                                (3000, 1, 0, 128), (2049, 0, 0, 129), (1300, 500, 0, 4),
+                                                (8300, 0, 0, 1000)])
 def test_sinks_split_over_their_queries(cuda, T, left, right, sinks, dtype):
     """Sequences long enough that the sinks' gradients are partial sums of several workgroups."""
     q, k, v, g = make(cuda, 2, T, 2, 1, 64, dtype, seed=T)
@@ -263,8 +264,9 @@ def test_long_sequence_properties(cuda):
         assert float(s.abs().max()) < 6 * (2 * T) ** 0.5 * 2 * max(HALF[dtype], 64 * U) * 3
 
 
-def test_graph_capture_and_streams(cuda):
-    q, k, v, g = make(cuda, 2, 1400, 4, 2, 64, torch.bfloat16)
+@pytest.mark.parametrize("D", [64, 128])
+def test_graph_capture_and_streams(cuda, D):
+    q, k, v, g = make(cuda, 2, 1400, 4, 2, D, torch.bfloat16)
     lengths = torch.tensor([1400, 900], device=cuda, dtype=torch.int32)
     how = dict(left=100, right=0, sinks=4, lengths=lengths)
     want = run(q, k, v, g, **how)
@@ -282,7 +284,7 @@ def test_graph_capture_and_streams(cuda):
             graphs.append((graph, run(q, k, v, g, **how)))
         graphs[-1] = (graph, graphs[-1][1])
     for seed in (1, 2, 3):
-        for t, new in zip((q, k, v, g), make(cuda, 2, 1400, 4, 2, 64, torch.bfloat16, seed)):
+        for t, new in zip((q, k, v, g), make(cuda, 2, 1400, 4, 2, D, torch.bfloat16, seed)):
             t.copy_(new)
         lengths.copy_(torch.tensor([1400 - 300 * seed, 900 + seed], dtype=torch.int32))
         for graph, _ in graphs:

@@ -229,3 +229,23 @@ def test_streams_and_graphs(cuda):
         e = ln.layer_norm_forward(x, 200, w, b)
         for p, q in zip(out + grads, e + ln.layer_norm_backward(gr, x, e[1], e[2], w, b)):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("D", [24, 700, 3000, 20001])
+def test_in_place_through_the_c_entry(cuda, D):
+    """y may take x's place, dx the gradient's."""
+    x, w, b, gr = _data(cuda, 70, D, torch.bfloat16, torch.float32)
+    y, mean, rstd = ln.layer_norm_forward(x, D, w, b)
+    want = ln.layer_norm_backward(gr, x, mean, rstd, w, b)
+    xi, gi = x.clone(), gr.clone()
+    dw, db = torch.empty_like(w), torch.empty_like(b)
+    nbytes = _lib.load().mn_layer_norm_ws_bytes(70, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cuda)
+    s = _lib.stream_ptr(cuda)
+    _lib.call("mn_layer_norm_bwd", gi.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), w.data_ptr(),
+              gi.data_ptr(), dw.data_ptr(), db.data_ptr(), 70, D, _lib.BF16, _lib.F32, ws.data_ptr(), nbytes, s)
+    for p, q in zip(want, (gi, dw, db)):
+        assert torch.equal(p, q)
+    _lib.call("mn_layer_norm_fwd", xi.data_ptr(), w.data_ptr(), b.data_ptr(), xi.data_ptr(), None, None, 70, D,
+              1e-5, _lib.BF16, _lib.F32, s)
+    assert torch.equal(xi, y)
