@@ -20,7 +20,22 @@
 // LDS tiles hold rows of D elements as they lie in memory; 16-byte chunk c of row r is stored at
 // chunk c ^ swz(r), which spreads both kinds of reads over all banks: rows (a lane reads 16 bytes
 // of its row) and transposed (16-bit: ds_read_b64_tr_b16 gives a lane four rows' values of its
-// column; fp32: plain 4-byte reads).
+// column; fp32: plain 4-byte reads).  Two buffers of two tiles: 64 KB at D = 128, two workgroups a
+// CU; rows of whole 16-byte chunks go from memory to LDS without registers, others through them
+// (D = 100 or 127: 2.5 times slower).
+//
+// Measured at T = 4099, causal, batch 8 of 16 heads, D = 128, bf16 (operations a visible pair needs
+// over time; a large bf16 matrix product of the library runs at 1160 TFLOP/s): forward 0.71 ms, 777
+// TFLOP/s; dq 0.91 ms, 911; dk and dv 1.62 ms, 682 (of the 8 D they need; they run 10 D).  The
+// matrix cores are busy 0.41, 0.49 and 0.41 of the time, LDS a sixth of it without conflicts: what is
+// left are waits of two waves per SIMD for LDS, for each other's products and at the barrier of a
+// tile.  fp32: 33 % to 60 % of the 154 TFLOP/s of a library product.
+//
+// Tried and not kept: 16 instead of 32 columns a wave (half the registers, twice the LDS reads: dk
+// and dv together at D = 128 in 0.62 ms where 32-wide halves take 0.50); dk and dv in one workgroup
+// (one wave per SIMD or spills: 0.98 ms); two waves sharing a wave's rows where there are few
+// workgroups (a CU's matrix cores have the same work: 24 us instead of 25 at batch 8, 197 tokens,
+// fp32); the row sums as a product with ones (no faster, and lse would carry P's rounding).
 #include <mutex>
 #include <type_traits>
 
@@ -601,7 +616,8 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_dq_kern
 // registers, in a fixed order.
 // dk and dv of a tile are two workgroups, which costs the scores twice (10 D instead of 8 D
 // operations a pair) and is faster: both at once are 2 x 64 accumulators and 2 x 32 registers of
-// keys and values at D = 128, which leaves no room for LDS reads in flight at two waves per SIMD.
+// keys and values at D = 128, which leaves no room for LDS reads in flight at two waves per SIMD
+// (T = 15808, window 1024, 16 heads on 4 of keys: 0.50 ms, in one workgroup 0.98).
 // Key tiles that hold sinks are seen by all later queries: their queries behind the window are
 // given to `nchunks` workgroups more (chunk queries each); all of a split tile's workgroups write
 // fp32 partial results, which attn_join_kernel adds in order.  Without that the one workgroup of

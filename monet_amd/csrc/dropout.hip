@@ -10,7 +10,8 @@
 // bit 31 of its second word set - are only generated where a high half equals the threshold's,
 // one element in 65536, since anywhere else the high half decides.  A word per element instead
 // would cost twice the multiplications, more time than the memory of 16-bit tensors takes.
-// Bound by memory: one read and one write per element, 16 bytes a lane and load.
+// Bound by memory: one read and one write per element, 16 bytes a lane and load: 36064 x 4096 bf16
+// in 102 us (5.8 TB/s; a copy of 1 GiB runs at 5.0), 10868 x 1023 fp32 in 15 us a direction.
 #include "elem.h"
 
 namespace {

@@ -13,6 +13,11 @@
 // Backward sums dw and db over a group's rows in registers, over a workgroup's groups in a fixed
 // order, and writes one partial row per workgroup; a second kernel adds those in a fixed order:
 // no atomics, the same bits every run.  All sums are fp32.
+//
+// 36064 rows x 2048, bf16 with fp32 weights: forward 68 us (4.4 TB/s), backward 93 us (4.7 TB/s)
+// and 4.5 us for the join; 36248 x 384, fp32: 21 us, 29 us (5.3 and 5.8 TB/s) and 4.5 us; a copy of
+// 1 GiB runs at 5.0 TB/s.  Without the next row's loads ahead, and with the sums through LDS, the
+// first took 107 and 145 us.
 #include "elem.h"
 
 namespace {
@@ -370,7 +375,7 @@ struct Shape {
 
 // The fewest lanes that hold a row (N = elements in 16 bytes).  A lane keeps up to 32 elements
 // forward, so that rows of 2048 need no exchange between waves (36064 x 2048 bf16: 68 us); backward
-// keeps five values for each, and 32 of them leave one wave per SIMD (114 us; 16: see below).
+// keeps five values for each, and 32 of them leave one wave per SIMD (114 us instead of 93).
 Shape shape_for(int64_t D, int N, bool backward) {
   for (int lanes = 8; lanes <= 64; lanes *= 2)
     if (D <= lanes * N) return {lanes, N};

@@ -12,6 +12,10 @@
 // quarter turns exactly (what is left is at most an eighth of a turn, 2^-28 turns after rounding
 // to fp32), so a position of a million is as accurate as position 1; sine and cosine of that rest
 // are fp32.
+// 184 x 196 tokens of 16 heads of 64, bf16: 34 us on operands from memory (4.3 TB/s), 27 us on ones
+// in the memory-side cache; 6916 tokens of 12 heads of 80, fp32: 14 us (3.8 TB/s; one round of
+// workgroups, half of it the wait for the table and the first loads).  With what a unit is worked
+// out for every element instead of once per lane the latter took 20 us.
 #include <math.h>
 
 #include "elem.h"
