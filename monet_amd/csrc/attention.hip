@@ -404,17 +404,18 @@ __device__ __forceinline__ void store_columns(T* row, const f32x16* acc, float f
 }
 
 // Which tile of which head (counting the batch) a workgroup has.  Each of the 8 XCDs runs a
-// contiguous range of (head, tile), so that neighbours find each other's keys in its L2.  Where
-// tiles differ in work (one side of the window open), a head's tiles are taken in pairs from both
-// ends, which gives any range the same share of long and short ones, and a range runs its long
-// ones first.
+// contiguous range of (key head, tile, query head), so that neighbours find each other's keys in
+// its L2 (T = 15808, window 1024, 4 heads to a key head: forward 178 us with the query heads one
+// after the other, 173 side by side).  Where tiles differ in work (one side of the window open),
+// query heads follow each other, and a head's tiles are taken in pairs from both ends, which gives
+// any range the same share of long and short ones; a range runs its long ones first.
 struct TileOf {
   int tile, head;
 };
-__device__ __forceinline__ TileOf tile_of(const Args& a, int tiles, bool last_is_long) {
+__device__ __forceinline__ TileOf tile_of(const Args& a, int tiles, int group, bool last_is_long) {
   if (!a.fold) {
-    const uint32_t slot = xcd_slot();
-    return {(int)(slot % tiles), (int)(slot / tiles)};
+    const uint32_t slot = xcd_slot(), k = slot / group;
+    return {(int)(k % tiles), (int)(k / tiles * group + slot % group)};
   }
   const uint32_t total = gridDim.x, xcd = blockIdx.x & 7u, j = blockIdx.x >> 3, rem = total & 7u;
   const uint32_t start = xcd * (total >> 3) + (xcd < rem ? xcd : rem), n = (total >> 3) + (xcd < rem ? 1 : 0);
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_fwd_ker
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const TileOf me = tile_of(a, a.tiles, a.left > a.right);
+  const TileOf me = tile_of(a, a.tiles, a.group, a.left > a.right);
   const int tile = me.tile, h = me.head % a.Hq, b = me.head / a.Hq;
   const int len = length_of(a, b);
   const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_dq_kern
   typedef Tile<T, DP, R> Ti;
   typedef typename Mma<T>::frag frag;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const TileOf me = tile_of(a, a.tiles, a.left > a.right);
+  const TileOf me = tile_of(a, a.tiles, a.group, a.left > a.right);
   const int tile = me.tile, h = me.head % a.Hq, b = me.head / a.Hq;
   const int len = length_of(a, b);
   const int wave = threadIdx.x / MN_WAVE, lane = threadIdx.x % MN_WAVE;
@@ -631,7 +632,7 @@ __device__ __forceinline__ KeyWork key_work(const Args& a) {
   KeyWork w;
   // the extra workgroups of the sinks stand evenly between the others
   const int extra = a.sink_tiles * a.nchunks, items = a.tiles + extra;
-  const TileOf me = tile_of(a, 2 * items, a.right > a.left);
+  const TileOf me = tile_of(a, 2 * items, 1, a.right > a.left);
   const int item = me.tile / 2;
   w.is_dk = me.tile % 2 == 0;
   w.hk = me.head % a.Hkv;
@@ -813,33 +814,40 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_dkv_ker
 // Adds the partial results of the sinks in order: one thread per element.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(const Args a, int64_t total) {
-  const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (e >= total) return;
-  const int64_t per_tile = (int64_t)a.sink_rows * a.D;
-  const int64_t in_tile = e % per_tile, which = e / per_tile % 2, tile = e / per_tile / 2 % a.sink_tiles;
-  const int64_t bh = e / per_tile / 2 / a.sink_tiles;
-  const int64_t j = tile * kQueries + in_tile / a.D, b = bh / a.Hkv, hk = bh % a.Hkv;
-  if (j >= a.sinks) return;
-  const float* p = a.parts + ((bh * a.sink_tiles + tile) * (a.nchunks + 1) * 2 + which) * per_tile + in_tile;
-  float s = 0.f;
-  if (j < length_of(a, (int)b)) {
+  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kThreads) {
+    const int64_t per_tile = (int64_t)a.sink_rows * a.D;
+    const int64_t in_tile = e % per_tile, which = e / per_tile % 2, tile = e / per_tile / 2 % a.sink_tiles;
+    const int64_t bh = e / per_tile / 2 / a.sink_tiles;
+    const int64_t j = tile * kQueries + in_tile / a.D, b = bh / a.Hkv, hk = bh % a.Hkv;
+    if (j >= a.sinks) continue;
+    const float* p = a.parts + ((bh * a.sink_tiles + tile) * (a.nchunks + 1) * 2 + which) * per_tile + in_tile;
+    float s = 0.f;
+    if (j < length_of(a, (int)b)) {
 #pragma unroll 8
-    for (int c = 0; c <= a.nchunks; ++c) s += p[(int64_t)c * 2 * per_tile];
+      for (int c = 0; c <= a.nchunks; ++c) s += p[(int64_t)c * 2 * per_tile];
+    }
+    T* out = (T*)(which ? a.dv : a.dk);
+    out[((b * a.T + j) * a.Hkv + hk) * a.D + in_tile % a.D] = (T)s;
   }
-  T* out = (T*)(which ? a.dv : a.dk);
-  out[((b * a.T + j) * a.Hkv + hk) * a.D + in_tile % a.D] = (T)s;
 }
 
 // ------------------------------------------------------------------------------- host side
+// Workgroups of a launch: threads are counted in 32 bits, and dk and dv take up to six workgroups for
+// one of the others.  A larger batch is run in parts, one after the other.
+constexpr int64_t kMaxGroups = ((1ll << 32) - 1) / kThreads / 6;
+int64_t batch_of_launch(const mn_attention* d) {
+  const int64_t tiles = (d->T + kQueries - 1) / kQueries, most = kMaxGroups / (tiles * d->Hq);
+  return d->B < most ? d->B : most;
+}
+
 int check(const mn_attention* d) {
   if (!d || d->B < 0 || d->T < 0 || d->Hq <= 0 || d->Hkv <= 0 || d->D <= 0) return MN_EINVAL;
   if (d->Hq % d->Hkv || d->left < -1 || d->right < -1 || d->sinks < 0) return MN_EINVAL;
   if (!(d->scale > 0.f) || d->scale > 1e30f) return MN_EINVAL;
   if (d->D > kMaxD || d->T >= (1 << 28)) return MN_EUNSUPPORTED;
-  // one workgroup per tile, head and entry, counted in 31 bits (dk and dv: at most six times that)
   const int64_t tiles = (d->T + kQueries - 1) / kQueries;
-  if (d->B >= (1 << 28) || d->Hq >= (1 << 20) || (tiles && d->B * d->Hq > (1ll << 28) / tiles))
-    return MN_EUNSUPPORTED;
+  if (d->B >= (1 << 28) || d->Hq >= (1 << 20)) return MN_EUNSUPPORTED;
+  if (tiles && (d->Hq > kMaxGroups / tiles || d->B * d->Hq > (1ll << 28) / tiles)) return MN_EUNSUPPORTED;
   return MN_OK;
 }
 
@@ -907,6 +915,19 @@ int for_width(int D, bool direct, F f) {
   return direct ? f(Int<128, true>()) : f(Int<128, false>());
 }
 
+// f(the operator on a part of the batch, the part's first entry) until the batch is through.
+template <typename F>
+int in_parts(const mn_attention* desc, F f) {
+  mn_attention d = *desc;
+  const int64_t part = batch_of_launch(desc);
+  for (int64_t b0 = 0; b0 < desc->B; b0 += part) {
+    d.B = desc->B - b0 < part ? desc->B - b0 : part;
+    const int st = f(&d, b0);
+    if (st != MN_OK) return st;
+  }
+  return MN_OK;
+}
+
 // Loads straight to LDS move 16-byte chunks: rows have to start on 16 bytes and be whole chunks.
 bool direct_rows(const void* p, const int64_t* stride, const mn_attention* d, int bytes) {
   const int64_t n = 16 / bytes;
@@ -948,67 +969,80 @@ bool mn_attention_init() {
 
 extern "C" {
 
-int mn_attention_fwd(const mn_attention* d, const void* q, const void* k, const void* v, const int32_t* lengths,
+int mn_attention_fwd(const mn_attention* desc, const void* q, const void* k, const void* v, const int32_t* lengths,
                      void* out, float* lse, int dtype, mn_stream_t stream) {
-  const int st = check(d);
+  const int st = check(desc);
   if (st != MN_OK) return st;
   return mn_for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (d->B == 0 || d->T == 0) return (int)MN_OK;
+    if (desc->B == 0 || desc->T == 0) return (int)MN_OK;
     if (!q || !k || !v || !out || !lse) return (int)MN_EINVAL;
-    Args a = args_for(d);
-    a.q = q; a.k = k; a.v = v; a.o = out; a.lse = lse; a.lengths = lengths;
-    const unsigned grid = (unsigned)(a.tiles * d->Hq * d->B);
-    const bool direct = direct_rows(k, a.sk, d, sizeof(T)) && direct_rows(v, a.sv, d, sizeof(T));
-    return for_width(d->D, direct, [&](auto w) {
-      constexpr int DP = decltype(w)::value, lds = kLdsQ<T, DP>;
-      constexpr bool DIRECT = decltype(w)::direct;
-      attn_fwd_kernel<T, DP, DIRECT><<<grid, kThreads, lds, mn_stream(stream)>>>(a);
-      return mn_launch_status();
+    return in_parts(desc, [&](const mn_attention* d, int64_t b0) {
+      Args a = args_for(d);
+      const int64_t tokens = b0 * d->T * d->Hq;
+      a.q = (const T*)q + b0 * a.sq[0]; a.k = (const T*)k + b0 * a.sk[0]; a.v = (const T*)v + b0 * a.sv[0];
+      a.o = (T*)out + tokens * d->D; a.lse = lse + tokens; a.lengths = lengths ? lengths + b0 : nullptr;
+      const unsigned grid = (unsigned)(a.tiles * d->Hq * d->B);
+      const bool direct = direct_rows(a.k, a.sk, desc, sizeof(T)) && direct_rows(a.v, a.sv, desc, sizeof(T));
+      return for_width(d->D, direct, [&](auto w) {
+        constexpr int DP = decltype(w)::value, lds = kLdsQ<T, DP>;
+        constexpr bool DIRECT = decltype(w)::direct;
+        attn_fwd_kernel<T, DP, DIRECT><<<grid, kThreads, lds, mn_stream(stream)>>>(a);
+        return mn_launch_status();
+      });
     });
   });
 }
 
-size_t mn_attention_bwd_ws_bytes(const mn_attention* d) {
-  if (check(d) != MN_OK) return 0;
+size_t mn_attention_bwd_ws_bytes(const mn_attention* desc) {
+  if (check(desc) != MN_OK || desc->T == 0) return 0;
+  mn_attention d = *desc;
+  d.B = batch_of_launch(desc);   // (parts of the batch take turns with it)
   Args a = {};
-  split_for(d, &a);
-  return ((size_t)d->B * d->Hq * d->T + parts_floats(d, a)) * sizeof(float);
+  split_for(&d, &a);
+  return ((size_t)d.B * d.Hq * d.T + parts_floats(&d, a)) * sizeof(float);
 }
 
-int mn_attention_bwd(const mn_attention* d, const void* grad, const void* q, const void* k, const void* v,
+int mn_attention_bwd(const mn_attention* desc, const void* grad, const void* q, const void* k, const void* v,
                      const void* out, const float* lse, const int32_t* lengths, void* dq, void* dk, void* dv,
                      int dtype, void* ws, size_t ws_bytes, mn_stream_t stream) {
-  const int st = check(d);
+  const int st = check(desc);
   if (st != MN_OK) return st;
   return mn_for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (d->B == 0 || d->T == 0) return (int)MN_OK;
+    if (desc->B == 0 || desc->T == 0) return (int)MN_OK;
     if (!grad || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return (int)MN_EINVAL;
-    if (!ws || ws_bytes < mn_attention_bwd_ws_bytes(d) || !mn_aligned(ws, 4)) return (int)MN_EINVAL;
-    Args a = args_for(d);
-    a.q = q; a.k = k; a.v = v; a.out = out; a.grad = grad; a.lse = const_cast<float*>(lse);
-    a.dq = dq; a.dk = dk; a.dv = dv; a.lengths = lengths;
-    a.delta = (float*)ws;
-    a.parts = a.delta + (size_t)d->B * d->Hq * d->T;
-    split_for(d, &a);
-    hipStream_t s = mn_stream(stream);
-    const bool direct = direct_rows(k, a.sk, d, sizeof(T)) && direct_rows(v, a.sv, d, sizeof(T)) &&
-                        direct_rows(q, a.sq, d, sizeof(T)) && mn_aligned(grad, 16) &&
-                        (int64_t)d->Hq * d->D < (1 << 22);
-    const int rc = for_width(d->D, direct, [&](auto w) {
-      constexpr bool DIRECT = decltype(w)::direct;
-      constexpr int DP = decltype(w)::value, lds_q = kLdsQ<T, DP>, lds_kv = kLdsKv<T, DP>;
-      if (lds_kv > 65536 && !mn_attention_init()) return (int)MN_ELAUNCH;
-      attn_dq_kernel<T, DP, DIRECT><<<(unsigned)(a.tiles * d->Hq * d->B), kThreads, lds_q, s>>>(a);
-      const unsigned items = (unsigned)(a.tiles + a.sink_tiles * a.nchunks);
-      attn_dkv_kernel<T, DP, DIRECT><<<(unsigned)(2 * items * d->Hkv * d->B), kThreads, lds_kv, s>>>(a);
+    if (!ws || ws_bytes < mn_attention_bwd_ws_bytes(desc) || !mn_aligned(ws, 4)) return (int)MN_EINVAL;
+    return in_parts(desc, [&](const mn_attention* d, int64_t b0) {
+      Args a = args_for(d);
+      const int64_t tokens = b0 * d->T * d->Hq, key_tokens = b0 * d->T * d->Hkv;
+      a.q = (const T*)q + b0 * a.sq[0]; a.k = (const T*)k + b0 * a.sk[0]; a.v = (const T*)v + b0 * a.sv[0];
+      a.out = (const T*)out + tokens * d->D; a.grad = (const T*)grad + tokens * d->D;
+      a.lse = const_cast<float*>(lse) + tokens; a.dq = (T*)dq + tokens * d->D;
+      a.dk = (T*)dk + key_tokens * d->D; a.dv = (T*)dv + key_tokens * d->D;
+      a.lengths = lengths ? lengths + b0 : nullptr;
+      a.delta = (float*)ws;
+      a.parts = a.delta + (size_t)d->B * d->Hq * d->T;
+      split_for(d, &a);
+      hipStream_t s = mn_stream(stream);
+      const bool direct = direct_rows(a.k, a.sk, desc, sizeof(T)) && direct_rows(a.v, a.sv, desc, sizeof(T)) &&
+                          direct_rows(a.q, a.sq, desc, sizeof(T)) && mn_aligned(grad, 16) &&
+                          (int64_t)d->Hq * d->D < (1 << 22);
+      const int rc = for_width(d->D, direct, [&](auto w) {
+        constexpr bool DIRECT = decltype(w)::direct;
+        constexpr int DP = decltype(w)::value, lds_q = kLdsQ<T, DP>, lds_kv = kLdsKv<T, DP>;
+        if (lds_kv > 65536 && !mn_attention_init()) return (int)MN_ELAUNCH;
+        attn_dq_kernel<T, DP, DIRECT><<<(unsigned)(a.tiles * d->Hq * d->B), kThreads, lds_q, s>>>(a);
+        const unsigned items = (unsigned)(a.tiles + a.sink_tiles * a.nchunks);
+        attn_dkv_kernel<T, DP, DIRECT><<<(unsigned)(2 * items * d->Hkv * d->B), kThreads, lds_kv, s>>>(a);
+        return mn_launch_status();
+      });
+      if (rc != MN_OK || !a.sink_tiles) return rc;
+      const int64_t total = d->B * d->Hkv * a.sink_tiles * 2 * a.sink_rows * d->D;
+      const int64_t groups = (total + kThreads - 1) / kThreads;
+      attn_join_kernel<T><<<(unsigned)(groups < (1 << 20) ? groups : 1 << 20), kThreads, 0, s>>>(a, total);
       return mn_launch_status();
     });
-    if (rc != MN_OK || !a.sink_tiles) return rc;
-    const int64_t total = d->B * d->Hkv * a.sink_tiles * 2 * a.sink_rows * d->D;
-    attn_join_kernel<T><<<(unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, total);
-    return mn_launch_status();
   });
 }
 

@@ -295,6 +295,7 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
 
 // ------------------------------------------------ rows too long for a workgroup's registers
 constexpr int kLongThreads = 1024;
+constexpr int64_t kLongRows = ((1ll << 32) - 1) / kLongThreads;   // threads of a launch: 32 bits
 
 template <typename T, typename W>
 __global__ __launch_bounds__(kLongThreads) void ln_fwd_long_kernel(
@@ -425,14 +426,14 @@ int fwd(const void* x, const void* w, const void* b, void* y, float* mean, float
   const float dim = (float)D;
   const Shape s = shape_for(D, Vec16<T>::N, false);
   if (!s.lanes) {
-    if (rows >= (1ll << 31)) return MN_EUNSUPPORTED;
+    if (rows > kLongRows) return MN_EUNSUPPORTED;
     ln_fwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
         (const T*)x, (const W*)w, (const W*)b, (T*)y, mean, rstd, D, dim, eps);
     return mn_launch_status();
   }
   return for_shape<Vec16<T>::N, false>(s, [&](auto cfg) {
     using C = decltype(cfg);
-        const int64_t want = (rows + C::groups - 1) / C::groups;
+    const int64_t want = (rows + C::groups - 1) / C::groups;
     const unsigned grid = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
     ln_fwd_kernel<T, W, C::lanes, C::ne><<<grid, C::threads, 0, st>>>(
         (const T*)x, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows, D, dim, eps);
@@ -447,7 +448,7 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
   const Shape s = shape_for(D, Vec16<T>::N, true);
   int nparts = 0;
   if (!s.lanes) {
-    if (rows >= (1ll << 31) || (D + 255) / 256 >= (1ll << 31)) return MN_EUNSUPPORTED;
+    if (rows > kLongRows) return MN_EUNSUPPORTED;
     // (before dx, which may take the gradient's place)
     if (dw || db) {
       nparts = parts_for(rows, D, Vec16<T>::N);
@@ -460,7 +461,7 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
   } else {
     const int rc = for_shape<Vec16<T>::N, true>(s, [&](auto cfg) {
       using C = decltype(cfg);
-            const int64_t want = (rows + C::groups - 1) / C::groups;
+      const int64_t want = (rows + C::groups - 1) / C::groups;
       const int most = parts_for(rows, D, Vec16<T>::N);
       const unsigned grid = (unsigned)(want < most ? want : most);
       const bool join = grid > 1 && (dw || db);

@@ -197,7 +197,8 @@ int mn_rotary(const mn_rotary_desc* d, const void* x, const void* positions, voi
   while ((a.B + bchunk - 1) / bchunk > 65535 && a.spb == 0) bchunk *= 2;
   const int64_t most = token_elems ? (1ll << 31) / (tok * token_elems) - 1 : bchunk;
   if (bchunk > most) bchunk = most;
-  if ((a.B + bchunk - 1) / bchunk > 65535) return MN_EUNSUPPORTED;
+  // (threads of a launch are counted in 32 bits)
+  if ((a.B + bchunk - 1) / bchunk > 65535 || tblocks > ((1ll << 32) - 1) / kThreads) return MN_EUNSUPPORTED;
   a.bchunk = (int)(bchunk < a.B ? bchunk : a.B);
   return mn_for_dtype(dtype, [&](auto t) {
     using T = decltype(t);

@@ -1,4 +1,5 @@
-"""Tensors of more than 2^31 elements: the last rows, tokens and elements are where they belong."""
+"""Tensors of more than 2^31 elements and batches of more workgroups than a launch takes: the last
+rows, tokens, elements and sequences are where they belong."""
 import pytest
 import torch
 
@@ -65,3 +66,22 @@ def test_attention(cuda):
     for a, b in ((dq, cq), (dk, ck), (dv, cv)):
         scale = float(b.float().abs().max())
         assert float((a[:, -800:].float() - b[:, -800:].float()).abs().max()) < 8 * 2.0 ** -8 * scale
+
+
+def test_attention_of_more_workgroups_than_a_launch_takes(cuda):
+    """Many short sequences: a batch that is run in parts.  A sequence's result does not depend on
+    the batch around it, so small batches taken out of it give the same bits."""
+    B, T, H, K, D = 720_000, 3, 8, 4, 8     # a part is at most 2^32 / 256 / 6 / 8 = 349 525 entries
+    q = torch.randn(B, T, H, D, device=cuda, dtype=torch.float16)
+    k, v = (torch.randn(B, T, K, D, device=cuda, dtype=torch.float16) for _ in range(2))
+    lengths = torch.randint(0, T + 1, (B,), device=cuda, dtype=torch.int32)
+    how = dict(left=1, right=0, sinks=1)
+    fwd, bwd = lm_ops.attention.window_attention_forward, lm_ops.attention.window_attention_backward
+    out, lse = fwd(q, k, v, lengths=lengths, **how)
+    grads = bwd(q, q, k, v, out, lse, lengths=lengths, **how)
+    for b in (0, 349_500, 699_000, B - 100):
+        cut = lambda t: t[b:b + 100]
+        o, l = fwd(cut(q), cut(k), cut(v), lengths=cut(lengths), **how)
+        assert torch.equal(cut(out), o) and torch.equal(cut(lse), l), b
+        for name, a, c in zip("qkv", grads, bwd(cut(q), cut(q), cut(k), cut(v), o, l, lengths=cut(lengths), **how)):
+            assert torch.equal(cut(a), c), (b, name)

@@ -143,6 +143,9 @@ def test_attention_workspace():
         kept = sinks if sinks < 128 else (sinks + 127) // 128 * 128
         assert parts % (key * kept) == 0 and 2 <= parts // (key * kept) <= 129, (T, left, sinks)
     assert size(T=2000, left=10, sinks=300) == rows * 2000   # more than an eighth of the keys
+    # a batch beyond a launch (2^32 threads, six workgroups to a tile and head) shares one part's
+    part = ((1 << 32) - 1) // 256 // 6 // (4 * 3)
+    assert size(B=part, sinks=0) == size(B=part + 1, sinks=0) == part * 4 * 300 * 4
 
 
 def test_operators_refuse_cpu_tensors():
