@@ -454,7 +454,7 @@ int mn_conv_bwd_weight_bias(const mn_conv2d* g, const void* dy, const void* x, v
 
 /* ------------------------------------------------------- transformer block --
  * The operators between the linear layers of a transformer block.  The
- * reference has none of them ; they follow the contract of its
+ * reference has none of them; they follow the contract of its
  * operator classes (monet/lm_ops/base.py:2-53), in which a backward
  * names the few tensors it needs kept.
  *
@@ -490,7 +490,8 @@ int mn_dropout(const void* x, void* y, int64_t n, double p, const uint64_t* stat
  * (of `axes`, at most 3) turns sections[a] pairs; pair i of axis a, i-th of the axis and k-th of
  * all n = sum(sections), by the angle pos[a, b, t] * base^(-i / sections[a]), or base^(-k / n) if
  * `joint`.  Pairs are elements (k, k + n), or (2k, 2k + 1) if `interleaved`; elements from 2n on
- * are copied.  n <= 128, H * D < 2^24.  inverse != 0 turns back: the backward pass. */
+ * are copied.  n <= 128, H * D < 2^24; positions of their own (pos_stride[1] != 0) for at most
+ * 65535 entries.  inverse != 0 turns back: the backward pass. */
 #define MN_POS_I64 0
 #define MN_POS_I32 1
 #define MN_POS_F32 2
@@ -511,7 +512,9 @@ int mn_rotary(const mn_rotary_desc* d, const void* x, const void* positions, voi
  *     j <= i + right  and  (j >= i - left  or  j < sinks)  and  i, j < lengths[b];
  * left / right = -1: no limit; right = 0: nothing later.  `lengths` (int32 [B], device) may be
  * NULL (T everywhere); tokens from lengths[b] on are never read as keys, and their own outputs
- * and gradients are zeros (lse -inf), whatever their memory holds.
+ * and gradients are zeros (lse -inf), whatever their memory holds.  A NaN or infinity in a key or
+ * value inside the length may reach queries that do not see it (zero times NaN), as it does when a
+ * masked softmax is multiplied with v.
  * q [B, T, Hq, D], k and v [B, T, Hkv, D] with strides in elements (the last one is 1); every
  * other tensor is dense: out, grad, dq [B, T, Hq, D], dk, dv [B, T, Hkv, D], lse fp32 [B, Hq, T],
  * the natural logarithm of the sum of exp(scale * q k).  D <= 128, scale > 0.  16-bit types

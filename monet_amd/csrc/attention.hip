@@ -35,7 +35,9 @@
 // and dv together at D = 128 in 0.62 ms where 32-wide halves take 0.50); dk and dv in one workgroup
 // (one wave per SIMD or spills: 0.98 ms); two waves sharing a wave's rows where there are few
 // workgroups (a CU's matrix cores have the same work: 24 us instead of 25 at batch 8, 197 tokens,
-// fp32); the row sums as a product with ones (no faster, and lse would carry P's rounding).
+// fp32); the row sums as a product with ones (no faster, and lse would carry P's rounding); four
+// waves per SIMD instead of three at D = 64 (11 x 988 tokens: 48 us either way); the four waves of a
+// workgroup of sinks alone taking turns with its queries (15808 tokens: no faster, and spills).
 #include <mutex>
 #include <type_traits>
 

@@ -64,7 +64,8 @@ def window_attention_forward(q, k, v, left=-1, right=0, sinks=0, scale=None, len
 
     scale    of the scores, 1 / sqrt(head size) unless given
     lengths  int32 [batch] on the GPU: tokens of each padded sequence.  What lies behind them is
-             not read, and comes out as zeros (lse -inf)
+             not read, and comes out as zeros (lse -inf).  (A NaN inside a sequence may reach
+             every query of it, as in a product of a masked softmax with v.)
     out [batch, tokens, heads, head size] has q's type; lse [batch, heads, tokens] is fp32.
     """
     code, q, k, v, lengths, d = _describe(q, k, v, left, right, sinks, scale, lengths)
