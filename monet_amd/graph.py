@@ -287,19 +287,21 @@ class Graph:
                 if not connected and len(out.uses()) == 0:
                     continue  # side effect on a buffer (e.g. num_batches_tracked += 1)
                 args = []
-                for i in n.inputs():
+                for pos, i in enumerate(n.inputs()):
                     for iu in lists.get(i.unique(), [i.unique()]):
                         if iu in const:
                             args.append(ComputeNode.V(const[iu]))
                         elif iu in node_of:
                             src = g._nodes[node_of[iu]]
                             if iu not in tracked and isinstance(src, ComputeNode):
-                                # a parameter reshaped before use (e.g. weight.t() for addmm):
-                                # refer to the parameter itself
-                                for ii in i.node().inputs():
-                                    assert isinstance(g._nodes[node_of[ii.unique()]], (Input, Param))
-                                    args.append(ComputeNode.D(node_of[ii.unique()],
-                                                              ii.requires_grad()))
+                                # the transposed weight that addmm is given is the one value
+                                # computed from a parameter that its operator takes back to it
+                                if not (kind == 'aten::addmm' and pos == 2 and src.op == 'aten::t'):
+                                    raise ValueError(
+                                        '%s reads the result of %s, which depends on parameters and buffers '
+                                        'alone. A schedule does not run such operators: register the result '
+                                        'as a buffer, or compute it outside forward()' % (kind, src.op))
+                                args.append(src.args[0])
                             else:
                                 grad = True if isinstance(src, ComputeNode) and iu in tracked \
                                     else bool(i.requires_grad())

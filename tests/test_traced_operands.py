@@ -1,0 +1,63 @@
+"""What an operator of a traced model may read besides activations: parameters and buffers as they
+are.  Values computed from them inside forward() are refused when the model is traced; a schedule
+would otherwise hand the operator the parameter in their place.  No GPU."""
+import pytest
+import torch
+import torch.nn as nn
+
+from monet_amd import functional as MF
+from monet_amd.graph import Graph
+
+T, D = 8, 8
+
+
+class Net(nn.Module):
+    def __init__(self, f):
+        super().__init__()
+        self.f = f
+        self.register_buffer("positions", torch.stack([torch.arange(T), torch.arange(T)]))
+        self.register_buffer("scale", torch.tensor(3.0))
+        self.lin = nn.Linear(D, D)
+        self.square = nn.Parameter(torch.randn(D, D))
+
+    def forward(self, x):
+        return self.f(self, x)
+
+    def heads(self, x):
+        return self.lin(x).view(-1, T, 1, D)
+
+
+def trace(f, shape=(T, D)):
+    return Graph.create(Net(f), shape)
+
+
+def graph_ops(g):
+    return [n.op for n in g.nodes if hasattr(n, "op")]
+
+
+@pytest.mark.parametrize("name, f", [
+    ("neg", lambda s, x: MF.rotary(s.heads(x), -s.positions, (2, 2))),
+    ("slice", lambda s, x: MF.rotary(s.heads(x), s.positions[:, :T], (2, 2))),
+    ("float", lambda s, x: MF.rotary(s.heads(x), s.positions.float(), (2, 2))),
+    ("stack", lambda s, x: MF.rotary(s.heads(x), torch.stack([s.positions[0], s.positions[1]]), (2, 2))),
+    ("scale", lambda s, x: s.lin(x) * (-s.scale)),
+    ("linear of a transposed weight", lambda s, x: nn.functional.linear(x, s.square.t(), s.lin.bias)),
+    ("linear of exp", lambda s, x: nn.functional.linear(x, s.square.exp(), s.lin.bias)),
+    ("product with a transposed weight", lambda s, x: s.lin(x) * s.square.t()),
+    ("cat", lambda s, x: torch.cat([s.lin(x), s.lin(x) + (-s.scale)], 1)),
+])
+def test_functions_of_parameters_are_refused(name, f):
+    with pytest.raises(ValueError, match="parameters and buffers"):
+        trace(f)
+
+
+def test_parameters_as_they_are():
+    """What stays: parameters and buffers themselves, numbers, and the transposed weight of addmm."""
+    g = trace(lambda s, x: MF.rotary(s.heads(x), s.positions, (2, 2)))
+    assert graph_ops(g)[-1] == "monet::rotary"
+    assert graph_ops(trace(lambda s, x: s.lin(x) * s.scale)) == ["aten::linear", "aten::mul"]
+    assert graph_ops(trace(lambda s, x: s.lin(x) * 2)) == ["aten::linear", "aten::mul"]
+    g = trace(lambda s, x: torch.addmm(s.lin.bias, x, s.square.t()), (D,))
+    add = g.nodes[-1]
+    assert add.op == "aten::addmm" and list(g.nodes[add.args[2].index].shape) == [D, D]
+    assert not hasattr(g.nodes[add.args[2].index], "op") and add.args[2].requires_grad
