@@ -287,6 +287,7 @@ class Graph:
                 if not connected and len(out.uses()) == 0:
                     continue  # side effect on a buffer (e.g. num_batches_tracked += 1)
                 args = []
+                transposed_weight = False
                 for pos, i in enumerate(n.inputs()):
                     for iu in lists.get(i.unique(), [i.unique()]):
                         if iu in const:
@@ -302,12 +303,16 @@ class Graph:
                                         'alone. A schedule does not run such operators: register the result '
                                         'as a buffer, or compute it outside forward()' % (kind, src.op))
                                 args.append(src.args[0])
+                                transposed_weight = True
                             else:
                                 grad = True if isinstance(src, ComputeNode) and iu in tracked \
                                     else bool(i.requires_grad())
                                 args.append(ComputeNode.D(node_of[iu], grad))
                         else:
                             raise ValueError('Nodes %s disconnected' % repr(i))
+                if kind == 'aten::addmm' and not transposed_weight:
+                    raise ValueError('aten::addmm runs with the transposed of a parameter as its second '
+                                     'factor only (nn.Linear); got %s' % repr(n))
                 is_depthwise = False
                 if kind == "aten::_convolution":
                     assert isinstance(args[8], ComputeNode.V)

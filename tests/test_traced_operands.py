@@ -61,3 +61,13 @@ def test_parameters_as_they_are():
     add = g.nodes[-1]
     assert add.op == "aten::addmm" and list(g.nodes[add.args[2].index].shape) == [D, D]
     assert not hasattr(g.nodes[add.args[2].index], "op") and add.args[2].requires_grad
+
+
+@pytest.mark.parametrize("name, f", [
+    ("parameter", lambda s, x: torch.addmm(s.lin.bias, x, s.square)),
+    ("activation", lambda s, x: torch.addmm(s.scale, x, s.lin(x).t())),
+])
+def test_addmm_of_another_operand_is_refused(name, f):
+    """Its operator multiplies with the transposed of the parameter it is given."""
+    with pytest.raises(ValueError, match="transposed"):
+        trace(f, (D,))
