@@ -71,3 +71,15 @@ def test_addmm_of_another_operand_is_refused(name, f):
     """Its operator multiplies with the transposed of the parameter it is given."""
     with pytest.raises(ValueError, match="transposed"):
         trace(f, (D,))
+
+
+@pytest.mark.parametrize("name, f", [
+    ("arange", lambda s, x: MF.rotary(s.heads(x), torch.arange(T)[None], (4,))),
+    ("lengths", lambda s, x: MF.window_attention(s.heads(x), s.heads(x), s.heads(x),
+                                                 lengths=torch.full((23,), T, dtype=torch.int32))),
+    ("factors", lambda s, x: s.lin(x) * torch.arange(float(D))),
+])
+def test_tensors_made_in_forward_are_refused(name, f):
+    """The trace runs on the CPU: they would be constants there."""
+    with pytest.raises(ValueError, match="buffer"):
+        trace(f)
