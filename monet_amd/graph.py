@@ -97,6 +97,9 @@ class ComputeNode(Node):
 FUSED_BN_RELU = "monet::batch_norm_relu"
 FUSED_ADD_RELU = "monet::add_relu"
 FUSED_BN_ADD_RELU = "monet::batch_norm_add_relu"
+# tensor arguments that get no gradient: positions, lengths.  Computed from the data they would leave
+# the backward of what computed them without one.
+_NO_GRADIENT = {"monet::rotary": 1, "monet::window_attention": 3}
 _FUSABLE = {"aten::batch_norm": FUSED_BN_RELU, "aten::add_": FUSED_ADD_RELU, "aten::add": FUSED_ADD_RELU}
 
 
@@ -308,6 +311,10 @@ class Graph:
                                 args.append(src.args[0])
                                 transposed_weight = True
                             else:
+                                if isinstance(src, ComputeNode) and _NO_GRADIENT.get(kind) == pos:
+                                    raise ValueError('%s has no gradient for its argument %d, which must be the '
+                                                     'input, a parameter or a buffer; got the result of %s'
+                                                     % (kind, pos, src.op))
                                 grad = True if isinstance(src, ComputeNode) and iu in tracked \
                                     else bool(i.requires_grad())
                                 args.append(ComputeNode.D(node_of[iu], grad))

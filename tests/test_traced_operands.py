@@ -83,3 +83,13 @@ def test_tensors_made_in_forward_are_refused(name, f):
     """The trace runs on the CPU: they would be constants there."""
     with pytest.raises(ValueError, match="buffer"):
         trace(f)
+
+
+@pytest.mark.parametrize("name, f", [
+    ("positions", lambda s, x: MF.rotary(s.heads(x), x.permute(2, 0, 1), (1,) * 3)),
+    ("lengths", lambda s, x: MF.window_attention(s.heads(x), s.heads(x), s.heads(x), lengths=s.lin(x))),
+])
+def test_computed_positions_and_lengths_are_refused(name, f):
+    """Neither has a gradient to pass on, which the backward of what computed it would wait for."""
+    with pytest.raises(ValueError, match="no gradient"):
+        trace(f)
