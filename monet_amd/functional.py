@@ -21,9 +21,11 @@ _library.define("rotary(Tensor x, Tensor positions, int[] sections, float base, 
                 "bool interleaved) -> Tensor")
 _library.define("window_attention(Tensor q, Tensor k, Tensor v, Tensor? lengths, int left, int right, "
                 "int sinks, float? scale) -> Tensor")
-# what a trace needs: the shape (a copy, since an operator may not return its argument)
+# what a trace needs: the shape, dense as the operators' results are (a copy, since an operator may
+# not return its argument)
 for _name in ("dropout", "rotary", "window_attention"):
-    _library.impl(_name, lambda x, *rest: x.detach().clone(), "CompositeExplicitAutograd")
+    _library.impl(_name, lambda x, *rest: x.detach().clone(memory_format=torch.contiguous_format),
+                  "CompositeExplicitAutograd")
 
 
 def _recorded(x):

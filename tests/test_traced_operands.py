@@ -93,3 +93,16 @@ def test_computed_positions_and_lengths_are_refused(name, f):
     """Neither has a gradient to pass on, which the backward of what computed it would wait for."""
     with pytest.raises(ValueError, match="no gradient"):
         trace(f)
+
+
+def test_traced_outputs_are_dense():
+    """As those of the operators: a view of one is traced where it would run."""
+    def turned(s, x):
+        y = s.lin(x).view(-1, 2, T, D // 2).transpose(1, 2)        # [batch, tokens, heads, head size]
+        return y
+
+    for f in (lambda s, x: MF.window_attention(turned(s, x), turned(s, x), turned(s, x)),
+              lambda s, x: MF.rotary(turned(s, x), s.positions, (1, 1)),
+              lambda s, x: MF.dropout(turned(s, x), 0.5, True)):
+        g = trace(lambda s, x: f(s, x).view(-1, T, D))
+        assert graph_ops(g)[-1] == "aten::view" and g.nodes[-1].shape == [-1, T, D]
