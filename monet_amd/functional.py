@@ -47,10 +47,10 @@ class _Dropout(torch.autograd.Function):
 def dropout(x, p=0.5, training=True):
     """As `torch.nn.functional.dropout`, with 16 bytes kept for the backward pass instead of a mask.
     The elements that are dropped follow from torch's generator of x's device."""
-    if _recorded(x):
-        return torch.ops.monet.dropout(x, float(p), bool(training))
     if not 0.0 <= p <= 1.0:
         raise RuntimeError(f"the probability must lie between 0 and 1, got {p}")
+    if _recorded(x):
+        return torch.ops.monet.dropout(x, float(p), bool(training))
     if not training or p == 0:
         return x
     if not x.is_cuda:

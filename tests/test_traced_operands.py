@@ -106,3 +106,9 @@ def test_traced_outputs_are_dense():
               lambda s, x: MF.dropout(turned(s, x), 0.5, True)):
         g = trace(lambda s, x: f(s, x).view(-1, T, D))
         assert graph_ops(g)[-1] == "aten::view" and g.nodes[-1].shape == [-1, T, D]
+
+
+@pytest.mark.parametrize("p", [-0.5, 1.5, float("nan")])
+def test_traced_dropout_refuses_what_an_eager_one_refuses(p):
+    with pytest.raises(RuntimeError, match="between 0 and 1"):
+        trace(lambda s, x: MF.dropout(s.lin(x), p, True))
