@@ -105,6 +105,11 @@ class WindowAttention(OP):
     backward_storage = [InputStorage(0, 1, 2), OutputStorage()]
     params = None   # (lse, lengths, window)
 
+    @staticmethod
+    def state_bytes(node):
+        B, T, H, _ = node.shape
+        return 4 * B * T * H
+
     def forward(self, q, k, v, lengths, left, right, sinks, scale):
         with torch.no_grad():
             how = dict(left=left, right=right, sinks=sinks, scale=scale)

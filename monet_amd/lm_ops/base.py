@@ -63,6 +63,12 @@ class OP:
     # known by name.
     recompute_needs_params = False
 
+    @staticmethod
+    def state_bytes(node) -> int:
+        """Bytes of what `params` holds from the forward of graph node `node` to its backward and grows
+        with the batch (per sample and negative where a dimension of the node's shape is -1)."""
+        return 0
+
     def intermediate(self, *args, **kwargs):
         return None
 

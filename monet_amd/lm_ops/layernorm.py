@@ -102,6 +102,11 @@ class InputActLayerNorm(OP):
     backward_storage = InputStorage(0)
     params = None   # (mean, rstd, weight, bias, does the input need a gradient)
 
+    @staticmethod
+    def state_bytes(node):
+        normalized_shape = node.args[1].value
+        return 8 * math.prod(node.shape[:len(node.shape) - len(normalized_shape)])
+
     def forward(self, input_, normalized_shape, weight=None, bias=None, eps=1e-5, *rest):
         with torch.no_grad():
             y, mean, rstd = layer_norm_forward(input_, normalized_shape, weight, bias, eps)

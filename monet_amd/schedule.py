@@ -267,6 +267,7 @@ class Schedule(Graph):
                 _, op, k, argspec, with_int, restore, has_params, native, inplace_src = ins
                 if restore:
                     op.params = state[k]
+                state[k] = None
                 args = [v if not is_t else regs[v[0]].requires_grad_(v[1]) for is_t, v in argspec]
                 if with_int:
                     regs[k], ints[k] = op.forward(*args)
@@ -275,7 +276,7 @@ class Schedule(Graph):
                     regs[k] = op.forward(*args)
                 del args
                 if has_params:
-                    state[k] = op.params
+                    state[k], op.params = op.params, None   # (operators live on, states do not)
                 if native:
                     state[k] = op
                 if inplace_src >= 0:
@@ -334,6 +335,10 @@ class Schedule(Graph):
                 else:
                     outs = op.backward(grad, stored)
                 del grad, stored
+                if has_params:
+                    op.params = None
+                if last:
+                    state[k] = None
                 if not isinstance(outs, (list, tuple)):
                     outs = (outs,)
                 assert len(outs) == len(deps), \

@@ -41,7 +41,8 @@ class SolverNode:
         self.local_memory = -1      # their bytes
         self.mem = -1               # bytes of this node's output
         self.workspace_mem = []     # MB beyond inputs and outputs, per implementation / variant
-        self.fixed_mem = -1         # inputs + parameters (+ parameter gradients so far)
+        self.fixed_mem = -1         # inputs + parameters (+ parameter gradients so far) + states
+        self.state_mem = 0          # bytes of a forward operator's `params` that grow with the batch
         self.workspace_compute = []  # ms, per implementation / variant
         self.last_used = -1
         self.recompute_workspace_mem = []
@@ -140,7 +141,8 @@ class SolverInfo:
     def extract(self, graph: Graph, *args, cost_fn=None):
         """Build the solver graph and profile it.  `args` = (input, *parameters),
         indexed like the graph's nodes.  `cost_fn(n, op, bwd_op)` may replace the
-        GPU measurement; it returns (meminfo triple, computeinfo triple)."""
+        GPU measurement; it returns (meminfo triple, computeinfo triple) and, if the
+        plan is to count them, the operator's `state_bytes`."""
         if args and hasattr(args[0], "is_floating_point") and args[0].is_floating_point():
             self.elem_bytes = int(args[0].element_size())   # bf16 / fp16 models: 2
         for i, n in enumerate(graph.nodes):
@@ -178,6 +180,7 @@ class SolverInfo:
         self.get_conv_info()
         self.get_inplace_info()
         self.get_workspace_cost(graph, *args, cost_fn=cost_fn)
+        self.add_states()
         self.size = len(self.nodes)
         if self.data_dir is not None:
             with open(Path(self.data_dir) / ("si_" + self.data_path + ".pkl"), 'wb') as f:
@@ -318,6 +321,20 @@ class SolverInfo:
             for prm in self.nodes[i].stored:  # parameter gradients accumulate through the backward
                 self.nodes[i].fixed_mem += _nbytes(list(prm.shape), self.bs, self._eb())
 
+    def state_bytes(self, op, n):
+        """Bytes of what operator `op` of graph node `n` keeps beside tensors for its backward."""
+        nbytes = op.state_bytes(n)
+        return -nbytes * self.bs if nbytes < 0 else nbytes
+
+    def add_states(self):
+        """What operators keep beside tensors lives from the forward pass to their backward step."""
+        states = {i: self.nodes[i].state_mem for i in range(self.loss)}
+        left = sum(states.values())
+        for i, node in self.nodes.items():
+            node.fixed_mem += left
+            if i > self.loss and node.bwd_op == "ip_grad":
+                left -= states[self.bwd_to_fwd[i]]
+
     def get_conv_info(self):
         self.conv_list = {}
         convop = self._impls('aten::_convolution')[0]
@@ -368,6 +385,10 @@ class SolverInfo:
             for i in self.nodes:
                 for name, table in zip(fields, tables):
                     setattr(self.nodes[i], name, table[i])
+            for node in self.nodes.values():
+                if isinstance(node, BwdNode):
+                    self.nodes[node.fwd_id].state_mem = max(self.state_bytes(op, node.fwd_node)
+                                                            for op in self._impls(node.fwd_node.op))
             return
 
         if cost_fn is None:
@@ -375,7 +396,7 @@ class SolverInfo:
 
             def cost_fn(n, op, bwd_op):
                 common = (n, op, graph, self.bs, bwd_op, self.select_conv_algo, self.do_inplace)
-                return meminfo(*common, *args), computeinfo(*common, *args)
+                return meminfo(*common, *args), computeinfo(*common, *args), self.state_bytes(op, n)
 
         for i in sorted(self.nodes.keys(), reverse=True):
             node = self.nodes[i]
@@ -383,7 +404,8 @@ class SolverInfo:
                 b, n = node, node.fwd_node
                 fwd = self.nodes[self.bwd_to_fwd[i]]
                 for op_impl in self._impls(n.op):
-                    (fmem, bmem, fmem_re), (ftime, btime, ftime_re) = cost_fn(n, op_impl(), b.bwd_op)
+                    (fmem, bmem, fmem_re), (ftime, btime, ftime_re), *state = cost_fn(n, op_impl(), b.bwd_op)
+                    fwd.state_mem = max([fwd.state_mem] + state)
                     if self.select_conv_algo and self.bwd_to_fwd[i] in self.conv_list:
                         b.workspace_mem.extend(bmem)
                         b.workspace_compute.extend(btime)
