@@ -271,7 +271,9 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : 256) void ln_bwd_kernel(
 }
 
 // dw / db = the partial rows added up: 32 columns a workgroup, 32 slices of the partial rows,
-// joined in order.  blockIdx.y: 0 = dw, 1 = db.
+// joined in order.  blockIdx.y: 0 = dw, 1 = db.  (A launch counts its threads in 32 bits: the
+// workgroups of a very long row walk over the columns.)
+constexpr int64_t kJoinBlocks = 1 << 20;
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__ parts, W* dw, W* db,
                                                        int nparts, int64_t D) {
@@ -279,18 +281,21 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
   W* out = blockIdx.y ? db : dw;
   if (!out) return;
   const int c = threadIdx.x % 32, slice = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * 32 + c;
-  float s = 0.f;
-  if (col < D) {
+  for (int64_t col0 = (int64_t)blockIdx.x * 32; col0 < D; col0 += (int64_t)gridDim.x * 32) {
+    const int64_t col = col0 + c;
+    float s = 0.f;
+    if (col < D) {
 #pragma unroll 8
-    for (int p = slice; p < nparts; p += 32) s += parts[((int64_t)p * 2 + blockIdx.y) * D + col];
+      for (int p = slice; p < nparts; p += 32) s += parts[((int64_t)p * 2 + blockIdx.y) * D + col];
+    }
+    __syncthreads();   // the columns before have been read
+    lds[slice][c] = s;
+    __syncthreads();
+    // the slices of column `slice`, one a lane
+    s = lane_sum<32>(lds[c][slice]);
+    const int64_t mine = col0 + slice;
+    if (c == 0 && mine < D) out[mine] = (W)s;
   }
-  lds[slice][c] = s;
-  __syncthreads();
-  // the slices of column `slice`, one a lane
-  s = lane_sum<32>(lds[c][slice]);
-  const int64_t mine = (int64_t)blockIdx.x * 32 + slice;
-  if (c == 0 && mine < D) out[mine] = (W)s;
 }
 
 // ------------------------------------------------ rows too long for a workgroup's registers
@@ -472,8 +477,11 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
     });
     if (rc != MN_OK) return rc;
   }
-  if (nparts)
-    ln_join_kernel<W><<<dim3((unsigned)((D + 31) / 32), 2), 1024, 0, st>>>(parts, (W*)dw, (W*)db, nparts, D);
+  if (nparts) {
+    const int64_t blocks = (D + 31) / 32;
+    ln_join_kernel<W><<<dim3((unsigned)(blocks < kJoinBlocks ? blocks : kJoinBlocks), 2), 1024, 0, st>>>(
+        parts, (W*)dw, (W*)db, nparts, D);
+  }
   return mn_launch_status();
 }
 
