@@ -12,7 +12,7 @@
 // before they work on one.
 // Backward sums dw and db over a group's rows in registers, over a workgroup's groups in a fixed
 // order, and writes one partial row per workgroup; a second kernel adds those in a fixed order:
-// no atomics, the same bits every run.  All sums are fp32.
+// no atomics, the same bits every run.  Sums are fp32, of rows too long for registers 64 bits.
 // y may lie where x does and dx where g does: those pointers are not declared free of aliases.
 //
 // 36064 rows x 2048, bf16 with fp32 weights: forward 68 us (4.4 TB/s), backward 93 us (4.7 TB/s)
@@ -299,26 +299,41 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
 }
 
 // ------------------------------------------------ rows too long for a workgroup's registers
+// A thread adds D / 1024 terms here, and rows / 64 for dw and db: in 64 bits, since a chain of fp32
+// additions drifts by up to half a step of its sum with each.
 constexpr int kLongThreads = 1024;
 constexpr int64_t kLongRows = ((1ll << 32) - 1) / kLongThreads;   // threads of a launch: 32 bits
+
+// Sum over a workgroup; every thread gets it.
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int o = MN_WAVE / 2; o; o >>= 1) v += __shfl_xor(v, o, MN_WAVE);
+  __syncthreads();   // the previous sum has been read
+  if (threadIdx.x % MN_WAVE == 0) lds[threadIdx.x / MN_WAVE] = v;
+  __syncthreads();
+  v = 0.;
+#pragma unroll
+  for (int w = 0; w < kLongThreads / MN_WAVE; ++w) v += lds[w];
+  return v;
+}
 
 template <typename T, typename W>
 __global__ __launch_bounds__(kLongThreads) void ln_fwd_long_kernel(
     const T* x, const W* __restrict__ w, const W* __restrict__ b, T* y, float* __restrict__ mean_out,
-    float* __restrict__ rstd_out, int64_t D, float dim, float eps) {
-  __shared__ float lds[2 * kLongThreads / MN_WAVE];
+    float* __restrict__ rstd_out, int64_t D, double dim, float eps) {
+  __shared__ double lds[kLongThreads / MN_WAVE];
   const int64_t row = blockIdx.x;
   const T* xr = x + row * D;
   T* yr = y + row * D;
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < D; i += kLongThreads) s += (float)xr[i];
-  const float mu = group_sum<kLongThreads>(s, lds) / dim;
-  s = 0.f;
+  double s = 0.;
+  for (int64_t i = threadIdx.x; i < D; i += kLongThreads) s += (double)(float)xr[i];
+  const float mu = (float)(block_sum(s, lds) / dim);
+  s = 0.;
   for (int64_t i = threadIdx.x; i < D; i += kLongThreads) {
-    const float d = (float)xr[i] - mu;
+    const double d = (float)xr[i] - mu;
     s += d * d;
   }
-  const float r = 1.f / sqrtf(group_sum<kLongThreads>(s, lds) / dim + eps);
+  const float r = 1.f / sqrtf((float)(block_sum(s, lds) / dim) + eps);
   for (int64_t i = threadIdx.x; i < D; i += kLongThreads)
     yr[i] = (T)(((float)xr[i] - mu) * r * (w ? (float)w[i] : 1.f) + (b ? (float)b[i] : 0.f));
   if (threadIdx.x == 0) {
@@ -330,19 +345,17 @@ __global__ __launch_bounds__(kLongThreads) void ln_fwd_long_kernel(
 template <typename T, typename W>
 __global__ __launch_bounds__(kLongThreads) void ln_bwd_long_kernel(
     const T* g, const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
-    const W* __restrict__ w, T* dx, int64_t D, float dim) {
-  __shared__ float lds[2 * kLongThreads / MN_WAVE];
+    const W* __restrict__ w, T* dx, int64_t D, double dim) {
+  __shared__ double lds[kLongThreads / MN_WAVE];
   const int64_t row = blockIdx.x;
   const float mu = mean[row], r = rstd[row];
-  float s1 = 0.f, s2 = 0.f;
+  double a1 = 0., a2 = 0.;
   for (int64_t i = threadIdx.x; i < D; i += kLongThreads) {
     const float gw = (float)g[row * D + i] * (w ? (float)w[i] : 1.f);
-    s1 += gw;
-    s2 += gw * ((float)x[row * D + i] - mu) * r;
+    a1 += (double)gw;
+    a2 += (double)gw * (double)(((float)x[row * D + i] - mu) * r);
   }
-  group_sum2<kLongThreads>(s1, s2, lds);
-  s1 /= dim;
-  s2 /= dim;
+  const float s1 = (float)(block_sum(a1, lds) / dim), s2 = (float)(block_sum(a2, lds) / dim);
   for (int64_t i = threadIdx.x; i < D; i += kLongThreads) {
     const float gw = (float)g[row * D + i] * (w ? (float)w[i] : 1.f);
     dx[row * D + i] = (T)(r * (gw - s1 - ((float)x[row * D + i] - mu) * r * s2));
@@ -357,14 +370,14 @@ __global__ __launch_bounds__(256) void ln_cols_kernel(const T* __restrict__ g, c
                                                       float* __restrict__ parts, int64_t rows, int64_t D) {
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (col >= D) return;
-  float aw = 0.f, ab = 0.f;
+  double aw = 0., ab = 0.;
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     const float gg = (float)g[row * D + col];
-    aw += gg * ((float)x[row * D + col] - mean[row]) * rstd[row];
-    ab += gg;
+    aw += (double)gg * (double)(((float)x[row * D + col] - mean[row]) * rstd[row]);
+    ab += (double)gg;
   }
-  parts[((int64_t)blockIdx.y * 2) * D + col] = aw;
-  parts[((int64_t)blockIdx.y * 2 + 1) * D + col] = ab;
+  parts[((int64_t)blockIdx.y * 2) * D + col] = (float)aw;
+  parts[((int64_t)blockIdx.y * 2 + 1) * D + col] = (float)ab;
 }
 
 template <typename W>
@@ -432,7 +445,7 @@ int fwd(const void* x, const void* w, const void* b, void* y, float* mean, float
   if (!s.lanes) {
     if (rows > kLongRows) return MN_EUNSUPPORTED;
     ln_fwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
-        (const T*)x, (const W*)w, (const W*)b, (T*)y, mean, rstd, D, dim, eps);
+        (const T*)x, (const W*)w, (const W*)b, (T*)y, mean, rstd, D, (double)D, eps);
     return mn_launch_status();
   }
   return for_shape<Vec16<T>::N, false>(s, [&](auto cfg) {
@@ -461,7 +474,7 @@ int bwd(const void* g, const void* x, const float* mean, const float* rstd, cons
     }
     if (dx)
       ln_bwd_long_kernel<T, W><<<(unsigned)rows, kLongThreads, 0, st>>>(
-          (const T*)g, (const T*)x, mean, rstd, (const W*)w, (T*)dx, D, dim);
+          (const T*)g, (const T*)x, mean, rstd, (const W*)w, (T*)dx, D, (double)D);
   } else {
     const int rc = for_shape<Vec16<T>::N, true>(s, [&](auto cfg) {
       using C = decltype(cfg);
