@@ -105,12 +105,12 @@ int mn_dropout(const void* x, void* y, int64_t n, double p, const uint64_t* stat
     hipStream_t s = mn_stream(stream);
     const int64_t blocks = ((n + 7) / 8 + kThreads - 1) / kThreads;
     const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
-    if (p == 1.0) {   // nothing stays: 1 / (1 - p) does not exist, and is not needed
+    const double scaled = p * 4294967296.0 + 0.5;
+    if (scaled >= 4294967296.0) {   // no number reaches the threshold: nothing stays (p = 1 among them)
       zero_all_kernel<T><<<grid, kThreads, 0, s>>>((T*)y, n);
       return mn_launch_status();
     }
-    const double scaled = p * 4294967296.0 + 0.5;
-    const uint32_t threshold = scaled >= 4294967295.0 ? 0xFFFFFFFFu : (uint32_t)scaled;
+    const uint32_t threshold = (uint32_t)scaled;
     dropout_kernel<T><<<grid, kThreads, 0, s>>>((const T*)x, (T*)y, n, state, threshold,
                                                 (float)(1.0 / (1.0 - p)));
     return mn_launch_status();
