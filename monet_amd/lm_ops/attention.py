@@ -51,7 +51,9 @@ def _describe(q, k, v, left, right, sinks, scale, lengths):
             raise RuntimeError(f"lengths must hold one number per sequence, {B}, got {list(lengths.shape)}")
         lengths = lengths.contiguous()
     q, k, v = _rows(q), _rows(k), _rows(v)
-    d = _lib.AttentionDesc(B=B, T=T, Hq=Hq, Hkv=Hkv, D=D, left=left, right=right, sinks=sinks, scale=scale)
+    # (numbers beyond the sequence are all the same, and ctypes would keep the low 64 bits of any)
+    d = _lib.AttentionDesc(B=B, T=T, Hq=Hq, Hkv=Hkv, D=D, left=min(left, T), right=min(right, T),
+                           sinks=min(sinks, T), scale=scale)
     d.q_stride[:] = q.stride()[:3]
     d.k_stride[:] = k.stride()[:3]
     d.v_stride[:] = v.stride()[:3]
