@@ -461,7 +461,7 @@ int mn_conv_bwd_weight_bias(const mn_conv2d* g, const void* dy, const void* x, v
  * `dtype` is the type of activations and their gradients: MN_F32, MN_BF16 or
  * MN_F16, row-major (the channels-last rule of MN_BF16 above concerns
  * convolutions only).  Rows may start at any address that is a multiple of the
- * element size.  All sums are fp32; a result is rounded once. */
+ * element size.  Sums are fp32 or wider; a result is rounded once. */
 #define MN_F16 2
 
 /* y = (x - mean) * rstd * w + b per row of D elements; w, b may be NULL (1, 0).

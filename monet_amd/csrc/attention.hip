@@ -21,13 +21,15 @@
 // chunk c ^ swz(r), which spreads both kinds of reads over all banks: rows (a lane reads 16 bytes
 // of its row) and transposed (16-bit: ds_read_b64_tr_b16 gives a lane four rows' values of its
 // column; fp32: plain 4-byte reads).  Two buffers of two tiles: 64 KB at D = 128, two workgroups a
-// CU; rows of whole 16-byte chunks go from memory to LDS without registers, others through them
-// (D = 100 or 127: 2.5 times slower).
+// CU; rows of whole 16-byte chunks go from memory to LDS without registers, others through them:
+// 2.3 to 2.8 times slower (batch 2 of 16 heads, 4099 tokens, causal, bf16: D = 104 and 100 forward
+// 196 and 492 us, backward 666 and 1519 us; 128 and 127: 202 and 553, 672 and 1732 us).  Through
+// registers, 16-bit types spill 25 of them in dk / dv and 4 in dq at D = 97 .. 128.
 //
 // Measured at T = 4099, causal, batch 8 of 16 heads, D = 128, bf16 (operations a visible pair needs
-// over time; a large bf16 matrix product of the library runs at 1160 TFLOP/s): forward 0.71 ms, 777
-// TFLOP/s; dq 0.91 ms, 911; dk and dv 1.62 ms, 682 (of the 8 D they need; they run 10 D).  The
-// matrix cores are busy 0.41, 0.49 and 0.41 of the time, LDS a sixth of it without conflicts: what is
+// over time; a large bf16 matrix product of the library runs at 1160 TFLOP/s): forward 0.67 ms, 820
+// TFLOP/s; dq 0.89 ms, 925; dk and dv 1.54 ms, 716 (of the 8 D they need; they run 10 D).  The
+// matrix cores are busy 0.37, 0.43 and 0.41 of the time, LDS a sixth of it without conflicts: what is
 // left are waits of two waves per SIMD for LDS, for each other's products and at the barrier of a
 // tile.  fp32: 33 % to 60 % of the 154 TFLOP/s of a library product.
 //
@@ -407,10 +409,16 @@ __device__ __forceinline__ void store_columns(T* row, const f32x16* acc, float f
 
 // Which tile of which head (counting the batch) a workgroup has.  Each of the 8 XCDs runs a
 // contiguous range of (key head, tile, query head), so that neighbours find each other's keys in
-// its L2 (T = 15808, window 1024, 4 heads to a key head: forward 178 us with the query heads one
-// after the other, 173 side by side).  Where tiles differ in work (one side of the window open),
-// query heads follow each other, and a head's tiles are taken in pairs from both ends, which gives
-// any range the same share of long and short ones; a range runs its long ones first.
+// its L2 (T = 15808, window 1024, 4 heads to a key head: forward reads 304 MB past the L2 with the
+// query heads one after the other, 100 side by side).  Where tiles differ in work (one side of the
+// window open beyond a quarter of the sequence), `fold`: query heads follow each other, and a head's
+// tiles are taken in pairs from both ends, which gives any range the same share of long and short
+// ones; a range runs its long ones first.  Folded against not, us forward / backward, causal, 16 heads
+// on 4 of D = 128, bf16:
+//   15808 tokens   window T/16: 179/602, 170/601   T/4: 508/2001, 522/2039   none: 1108/4535, 1373/5590
+//   8 x 2048       window T/16: 74/203, 74/204     T/4: 104/354, 98/346      none: 178/694, 184/743
+//   2 x 4099       window T/16: 48/156, 44/125     T/4: 86/333, 87/308       none: 191/765, 183/756
+// (T/4 is where the long sequence starts to win; few workgroups lose up to 8 % by it.)
 struct TileOf {
   int tile, head;
 };
@@ -620,7 +628,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, DP>)) void attn_dq_kern
 // dk and dv of a tile are two workgroups, which costs the scores twice (10 D instead of 8 D
 // operations a pair) and is faster: both at once are 2 x 64 accumulators and 2 x 32 registers of
 // keys and values at D = 128, which leaves no room for LDS reads in flight at two waves per SIMD
-// (T = 15808, window 1024, 16 heads on 4 of keys: 0.50 ms, in one workgroup 0.98).
+// (T = 15808, window 1024, 16 heads on 4 of keys: 0.48 ms, in one workgroup 0.98).
 // Key tiles that hold sinks are seen by all later queries: their queries behind the window are
 // given to `nchunks` workgroups more (chunk queries each); all of a split tile's workgroups write
 // fp32 partial results, which attn_join_kernel adds in order.  Without that the one workgroup of

@@ -8,7 +8,8 @@ typedef _Float16 f16_t;
 
 // 16 bytes of T.  The alignment of one element is enough: rows of odd length and views that
 // start anywhere take the same 16-byte global accesses (the hardware splits the ones that cross
-// a line), so no kernel has an aligned and an unaligned variant.
+// a line), so that layer norm, dropout and rotary positions have one variant for all of them.
+// (Attention has two: loads straight to LDS need aligned 16-byte chunks.)
 template <typename T>
 struct Vec16 {
   static constexpr int N = 16 / (int)sizeof(T);

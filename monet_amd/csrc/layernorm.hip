@@ -6,19 +6,24 @@
 // Both passes are bound by memory: a row is read once, kept in registers (NE values per lane),
 // and written once.  The variance is taken around the mean in a second pass over the registers,
 // so a row far off zero loses nothing.  LANES lanes share a row: part of a wave for short rows
-// (several rows a wave), a wave up to 2048 elements, a workgroup above; the groups walk over the
-// rows with w and b in registers, so those are read once per group and not once per row (with
+// (several rows a wave), a wave up to 2048 elements forward and 1024 backward, a workgroup above, of
+// up to 1024 lanes and 16384 elements; the groups walk over the rows with w and b in registers, so those are read once per group and not once per row (with
 // fp32 weights next to 16-bit rows they are twice the bytes of the row), and load the next row
-// before they work on one.
+// before they work on one.  Longer rows are read again for each sum, an element a lane at a time.
 // Backward sums dw and db over a group's rows in registers, over a workgroup's groups in a fixed
 // order, and writes one partial row per workgroup; a second kernel adds those in a fixed order:
 // no atomics, the same bits every run.  Sums are fp32, of rows too long for registers 64 bits.
 // y may lie where x does and dx where g does: those pointers are not declared free of aliases.
 //
-// 36064 rows x 2048, bf16 with fp32 weights: forward 68 us (4.4 TB/s), backward 93 us (4.7 TB/s)
-// and 4.5 us for the join; 36248 x 384, fp32: 21 us, 29 us (5.3 and 5.8 TB/s) and 4.5 us; a copy of
-// 1 GiB runs at 5.0 TB/s.  Without the next row's loads ahead, and with the sums through LDS, the
+// 36064 rows x 2048, bf16 with fp32 weights: forward 68 us (4.4 TB/s), backward 92 us (4.8 TB/s)
+// and 5 us for the join; 36248 x 384, fp32: 22 us, 29 us (5.1 and 5.8 TB/s) and 4 us; a copy of
+// 1 GiB runs at 5.1 TB/s.  Without the next row's loads ahead, and with the sums through LDS, the
 // first took 107 and 145 us.
+// Wider rows are further from the copy.  Backward with 1024 lanes (8193 .. 16384 elements) has 128
+// registers a lane, does not fit and spills 83 to 117 of them to scratch memory.  bf16 with fp32
+// weights, forward / backward: 6000 x 8192 in 52 / 109 us (3.8 / 2.7 TB/s), 4096 x 12288 in 86 / 287
+// (2.4 / 1.1), 3000 x 16384 in 86 / 291 (2.3 / 1.0); in several passes over a row, 2000 x 16392 in
+// 67 / 106 (2.0 / 1.9) and 512 x 150528 in 165 / 359 (1.9 / 1.3).
 #include "elem.h"
 
 namespace {
