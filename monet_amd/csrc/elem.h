@@ -88,6 +88,32 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
+// The same for 64 bits and a whole wave: each half of a number moves like a float.
+__device__ __forceinline__ double from_halves(uint32_t lo, uint32_t hi) {
+  return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+template <int CTRL>
+__device__ __forceinline__ double plus_dpp(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xf, 0xf, true);
+  return v + from_halves((uint32_t)lo, (uint32_t)hi);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v = plus_dpp<0xB1>(v);
+  v = plus_dpp<0x4E>(v);
+  v = plus_dpp<0x141>(v);
+  v = plus_dpp<0x140>(v);
+  uint64_t b = (uint64_t)__double_as_longlong(v);
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  v = from_halves(lo[0], hi[0]) + from_halves(lo[1], hi[1]);
+  b = (uint64_t)__double_as_longlong(v);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  return from_halves(lo[0], hi[0]) + from_halves(lo[1], hi[1]);
+}
+
 // Calls f with a value of the element type that `dtype` names; MN_EUNSUPPORTED for others.
 template <typename F>
 static inline int mn_for_dtype(int dtype, F f) {

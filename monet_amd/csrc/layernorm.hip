@@ -23,7 +23,7 @@
 // registers a lane, does not fit and spills 83 to 117 of them to scratch memory.  bf16 with fp32
 // weights, forward / backward: 6000 x 8192 in 52 / 109 us (3.8 / 2.7 TB/s), 4096 x 12288 in 86 / 287
 // (2.4 / 1.1), 3000 x 16384 in 86 / 291 (2.3 / 1.0); in several passes over a row, 2000 x 16392 in
-// 67 / 106 (2.0 / 1.9) and 512 x 150528 in 165 / 359 (1.9 / 1.3).
+// 62 / 103 (2.1 / 1.9) and 512 x 150528 in 163 / 359 (1.9 / 1.3).
 #include "elem.h"
 
 namespace {
@@ -311,8 +311,7 @@ constexpr int64_t kLongRows = ((1ll << 32) - 1) / kLongThreads;   // threads of 
 
 // Sum over a workgroup; every thread gets it.
 __device__ __forceinline__ double block_sum(double v, double* lds) {
-#pragma unroll
-  for (int o = MN_WAVE / 2; o; o >>= 1) v += __shfl_xor(v, o, MN_WAVE);
+  v = wave_sum64(v);
   __syncthreads();   // the previous sum has been read
   if (threadIdx.x % MN_WAVE == 0) lds[threadIdx.x / MN_WAVE] = v;
   __syncthreads();
