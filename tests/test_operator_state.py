@@ -125,3 +125,14 @@ def test_the_executor_holds_no_more(mode, frac, monkeypatch):
         assert sum(alive.values()) == whole
         sched.backward(torch.ones_like(y))
         assert not alive and counted == 0
+
+
+def test_profiles_read_from_a_file_count_it(tmp_path):
+    """Costs that were written before (a file holds run times and workspaces) give the same plan."""
+    graph = Graph.create(Stack(), (T, WIDTH))
+    fixed = []
+    for _ in range(2):
+        si = SolverInfo(4, "stack", "normal", data_dir=tmp_path)
+        si.extract(graph, cost_fn=counted_cost(si))
+        fixed.append([n.fixed_mem for n in si.nodes.values()])
+    assert fixed[0] == fixed[1] and max(n.state_mem for n in si.nodes.values()) == 4 * 4 * HEADS * T
