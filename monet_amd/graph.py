@@ -295,8 +295,10 @@ class Graph:
                     for iu in lists.get(i.unique(), [i.unique()]):
                         if iu in const:
                             if isinstance(const[iu], torch.Tensor) and const[iu].dim() > 0:
-                                raise ValueError('%s reads a tensor made in forward(), which the trace holds as '
-                                                 'a constant on the CPU: register it as a buffer' % kind)
+                                raise ValueError('%s reads a tensor that is not in the state_dict (made in forward(), '
+                                                 'a plain attribute, a buffer that is not persistent), which the '
+                                                 'trace holds as a constant on the CPU: register it as a persistent '
+                                                 'buffer' % kind)
                             args.append(ComputeNode.V(const[iu]))
                         elif iu in node_of:
                             src = g._nodes[node_of[iu]]

@@ -19,6 +19,8 @@ class Net(nn.Module):
         self.register_buffer("scale", torch.tensor(3.0))
         self.lin = nn.Linear(D, D)
         self.square = nn.Parameter(torch.randn(D, D))
+        self.register_buffer("passing", torch.arange(T)[None], persistent=False)
+        self.attribute = torch.arange(T)[None]
 
     def forward(self, x):
         return self.f(self, x)
@@ -78,10 +80,12 @@ def test_addmm_of_another_operand_is_refused(name, f):
     ("lengths", lambda s, x: MF.window_attention(s.heads(x), s.heads(x), s.heads(x),
                                                  lengths=torch.full((23,), T, dtype=torch.int32))),
     ("factors", lambda s, x: s.lin(x) * torch.arange(float(D))),
+    ("buffer that is not persistent", lambda s, x: MF.rotary(s.heads(x), s.passing, (4,))),
+    ("attribute", lambda s, x: MF.rotary(s.heads(x), s.attribute, (4,))),
 ])
-def test_tensors_made_in_forward_are_refused(name, f):
+def test_tensors_outside_the_state_dict_are_refused(name, f):
     """The trace runs on the CPU: they would be constants there."""
-    with pytest.raises(ValueError, match="buffer"):
+    with pytest.raises(ValueError, match="persistent"):
         trace(f)
 
 
